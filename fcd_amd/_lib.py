@@ -57,7 +57,19 @@ class WgradDesc(C.Structure):
     ]
 
 
+class LayerNormDesc(C.Structure):
+    """Mirror of ``FcdLayerNormDesc``."""
+    _fields_ = [
+        ("rows", C.c_int64), ("cols", C.c_int64),
+        ("ld_x", C.c_int64), ("ld_res", C.c_int64), ("ld_gy", C.c_int64), ("ld_ggx", C.c_int64),
+        ("ld_out", C.c_int64), ("ld_ggy", C.c_int64),
+        ("seed", C.c_uint64), ("offset", C.c_uint64), ("rng", C.c_void_p), ("drop_p", C.c_double),
+        ("eps", C.c_float), ("act", C.c_float), ("dtype", C.c_int32), ("param_dtype", C.c_int32),
+    ]
+
+
 _P, _I, _F, _Z = C.c_void_p, C.c_int, C.c_float, C.c_size_t
+_L, _U = C.c_int64, C.c_uint64
 
 # name -> (restype, argtypes); every symbol declared in include/fcd_hip.h
 PROTOTYPES = {
@@ -136,6 +148,13 @@ PROTOTYPES = {
     "fcd_patch_batch": (_I, [_P, C.c_long, _I, _I, _I, _P, _P, _I, _P, _P, _P, _P]),
     "fcd_valid_minmax": (_I, [_P, _P, C.c_size_t, _P, _P]),
     "fcd_threshold_hist": (_I, [_P, _P, C.c_size_t, _P, _I, _P, _P]),
+    "fcd_layernorm_desc_bytes": (_I, []),
+    "fcd_layernorm_fwd": (_I, [C.POINTER(LayerNormDesc), _P, _P, _P, _P, _P, _P, _P, _P]),
+    "fcd_layernorm_workspace_bytes": (_Z, [C.POINTER(LayerNormDesc)]),
+    "fcd_layernorm_bwd": (_I, [C.POINTER(LayerNormDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _Z, _P]),
+    "fcd_layernorm_bwd2": (_I, [C.POINTER(LayerNormDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _Z, _P]),
+    "fcd_dropout": (_I, [_P, _P, _P, _L, _L, _L, _L, _L, _I, C.c_double, _U, _U, _P, _P]),
+    "fcd_dropout_take": (_I, [_P, _P, _U, _P]),
 }
 
 _lib: Optional[C.CDLL] = None
@@ -161,6 +180,9 @@ def load() -> C.CDLL:
         raise RuntimeError("fcd_amd: descriptor layouts of libfcd_hip.so and of this binding differ "
                            f"(FcdConvDesc {lib.fcd_conv_desc_bytes()} / {C.sizeof(ConvDesc)} bytes, "
                            f"FcdWgradDesc {lib.fcd_wgrad_desc_bytes()} / {C.sizeof(WgradDesc)} bytes)")
+    if lib.fcd_layernorm_desc_bytes() != C.sizeof(LayerNormDesc):
+        raise RuntimeError("fcd_amd: descriptor layouts of libfcd_hip.so and of this binding differ "
+                           f"(FcdLayerNormDesc {lib.fcd_layernorm_desc_bytes()} / {C.sizeof(LayerNormDesc)} bytes)")
     _lib = lib
     return lib
 

@@ -7,6 +7,7 @@ of 4 (pad channels are zero).
 from __future__ import annotations
 
 import ctypes as C
+import math
 from dataclasses import dataclass
 from typing import Optional
 
@@ -734,6 +735,218 @@ def instnorm_affine_batch(items, accumulate: bool) -> None:
             cols = [arr(*[ptr(it[k]) for it in part]) for k in range(3)]
             check(L.load().fcd_instnorm_affine_batch(cols[0], cols[1], cols[2], len(part), n, c, int(accumulate), stream()),
                   "instnorm_affine_batch")
+
+
+# --------------------------------------------------------------------------- #
+# layer norm over the last axis, dropout
+# --------------------------------------------------------------------------- #
+LN_EPS = 1e-5
+_DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # FCD_DT_*
+_U64 = (1 << 64) - 1
+
+
+def _rows(t: torch.Tensor, name: str):
+    """(rows, cols, row stride) of a tensor whose last axis is contiguous and whose other axes are evenly spaced."""
+    if t.dim() == 0:
+        raise RuntimeError(f"fcd_amd: {name} needs at least one axis")
+    if t.is_contiguous():
+        cols = t.shape[-1]
+        return (t.numel() // cols if cols else math.prod(t.shape[:-1])), cols, cols
+    shape, strides = t.shape, t.stride()
+    cols = shape[-1]
+    if cols > 1 and strides[-1] != 1:
+        raise RuntimeError(f"fcd_amd: the last axis of {name} must be contiguous")
+    rows, ld = 1, None
+    for n, st in zip(reversed(shape[:-1]), reversed(strides[:-1])):
+        if n == 1:
+            continue
+        if ld is None:
+            ld = st
+        elif st != rows * ld:
+            raise RuntimeError(f"fcd_amd: the rows of {name} must be evenly spaced (strides {tuple(strides)})")
+        rows *= n
+    return rows, cols, cols if ld is None else ld
+
+
+def _row_operand(t: torch.Tensor, name: str, like: torch.Tensor) -> int:
+    """Row stride of ``t``, which goes with ``like`` (same shape, type and device)."""
+    if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
+        raise RuntimeError(f"fcd_amd: {name} is {t.dtype} {tuple(t.shape)} on {t.device}, "
+                           f"expected {like.dtype} {tuple(like.shape)} on {like.device}")
+    return _rows(t, name)[2]
+
+
+def _require_here(t: torch.Tensor, name: str) -> None:
+    if not t.is_cuda:
+        raise RuntimeError(f"fcd_amd: {name} must live on the GPU (got {t.device}); the HIP path has no CPU fallback")
+    if t.get_device() != torch._C._cuda_getDevice():
+        raise RuntimeError(f"fcd_amd: {name} is on {t.device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+    if t.dtype not in _DT:
+        raise RuntimeError(f"fcd_amd: {name} must be float32, bfloat16 or float16 (got {t.dtype})")
+
+
+def _rng_words(p: float, rng, device):
+    """(seed, offset, device address) for the C calls."""
+    if not 0.0 <= p <= 1.0:
+        raise RuntimeError(f"fcd_amd: the dropout probability must be in [0, 1] (got {p})")
+    if p == 0.0:
+        return 0, 0, None
+    if rng is None:
+        raise RuntimeError("fcd_amd: dropout needs rng: (seed, offset) or what dropout_take returned")
+    if isinstance(rng, torch.Tensor):
+        if rng.dtype != torch.int64 or rng.numel() != 2 or not rng.is_contiguous() or rng.device != device:
+            raise RuntimeError("fcd_amd: a dropout rng tensor is two contiguous int64 words on the operands' device")
+        return 0, 0, rng.data_ptr()
+    seed, offset = rng
+    return int(seed) & _U64, int(offset) & _U64, None
+
+
+def dropout_state(seed: int, device, offset: int = 0) -> torch.Tensor:
+    """A generator's state on the device: (seed, next block).  :func:`dropout_take` hands out ranges of it."""
+    def signed(v):
+        v = int(v) & _U64
+        return v - (1 << 64) if v >> 63 else v
+    return torch.tensor([signed(seed), signed(offset)], dtype=torch.int64, device=device)
+
+
+def dropout_take(state: torch.Tensor, numel: int) -> torch.Tensor:
+    """The ``rng`` for ``numel`` elements; ``state`` moves on.  One tiny launch, no host synchronisation: inside a captured
+    graph every replay takes the next range.  Keep the returned tensor for the backward pass."""
+    if not state.is_cuda or state.dtype != torch.int64 or state.numel() != 2 or not state.is_contiguous():
+        raise RuntimeError("fcd_amd: a dropout state is two contiguous int64 words on the GPU (dropout_state)")
+    if state.get_device() != torch._C._cuda_getDevice():
+        raise RuntimeError(f"fcd_amd: the dropout state is on {state.device}, the current device is "
+                           f"cuda:{torch._C._cuda_getDevice()}")
+    if numel < 0:
+        raise RuntimeError("fcd_amd: dropout_take of a negative number of elements")
+    taken = torch.empty_like(state)
+    check(L.load().fcd_dropout_take(state.data_ptr(), taken.data_ptr(), (int(numel) + 7) // 8, stream()), "dropout_take")
+    return taken
+
+
+def dropout(x: torch.Tensor, p: float, rng, residual: Optional[torch.Tensor] = None,
+            out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``x * mask / (1 - p) (+ residual)``; the mask is a function of ``rng`` and the element's row-major index and is never
+    stored: the backward pass is the same call on the gradient (without ``residual``).  ``rng`` is ``(seed, offset)`` or
+    what :func:`dropout_take` returned; ``numel`` elements use ``ceil(numel / 8)`` offsets.  ``p`` is resolved to 2^-16.
+    float32, bfloat16, float16; rows may be strided; ``out`` may be ``x``."""
+    _require_here(x, "x")
+    rows, cols, ld = _rows(x, "x")
+    seed, offset, words = _rng_words(p, rng, x.device)
+    ld_r = 0 if residual is None else _row_operand(residual, "residual", x)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        ld_o = cols
+    else:
+        ld_o = _row_operand(out, "out", x)
+    check(L.load().fcd_dropout(x.data_ptr(), ptr(residual), out.data_ptr(), rows, cols, ld, ld_r, ld_o, _DT[x.dtype], p, seed,
+                               offset, words, stream()), "dropout")
+    return out
+
+
+def _ln_desc(x, gamma, beta, eps, act_slope, p, rng):
+    _require_here(x, "x")
+    d = L.LayerNormDesc()
+    d.rows, d.cols, d.ld_x = _rows(x, "x")
+    d.dtype = d.param_dtype = _DT[x.dtype]
+    if gamma is None and beta is None:
+        d.param_dtype = 0
+    for t, name in ((gamma, "gamma"), (beta, "beta")):
+        if t is not None:
+            if t.dtype not in (torch.float32, x.dtype) or t.device != x.device or t.numel() != d.cols or not t.is_contiguous():
+                raise RuntimeError(f"fcd_amd: {name} must be a contiguous float32 or {x.dtype} vector of {d.cols} elements "
+                                   f"on {x.device}")
+            d.param_dtype = _DT[t.dtype]
+    if gamma is not None and beta is not None and gamma.dtype != beta.dtype:
+        raise RuntimeError("fcd_amd: gamma and beta must have one type")
+    d.eps, d.act, d.drop_p = eps, act_slope, p
+    d.seed, d.offset, d.rng = _rng_words(p, rng, x.device)
+    return d
+
+
+def _ln_stat(t, name, d, x):
+    if t.dtype != torch.float32 or t.device != x.device or t.numel() != d.rows or not t.is_contiguous():
+        raise RuntimeError(f"fcd_amd: {name} must be a contiguous float32 vector of {d.rows} elements on {x.device}")
+    return t.data_ptr()
+
+
+def _ln_affine(gamma, beta, want_affine, dgamma, dbeta, accumulate, d, x):
+    """Gradient tensors of the affine parameters (given, fresh, or None) and the scratch their row sums need."""
+    if want_affine and dgamma is None and dbeta is None:
+        if accumulate:
+            raise RuntimeError("fcd_amd: accumulate needs dgamma / dbeta")
+        dgamma = None if gamma is None else torch.empty_like(gamma)
+        dbeta = None if beta is None else torch.empty_like(beta)
+    elif not want_affine:
+        dgamma = dbeta = None
+    for t, name in ((dgamma, "dgamma"), (dbeta, "dbeta")):
+        if t is not None and (_DT.get(t.dtype) != d.param_dtype or t.device != x.device or t.numel() != d.cols
+                              or not t.is_contiguous()):
+            raise RuntimeError(f"fcd_amd: {name} must be a contiguous vector of {d.cols} elements of the parameters' type")
+    ws = None
+    if dgamma is not None or dbeta is not None:
+        # a buffer of this call's own: inside a captured graph it belongs to that graph's memory
+        ws = torch.empty(L.load().fcd_layernorm_workspace_bytes(C.byref(d)), dtype=torch.uint8, device=x.device)
+    return dgamma, dbeta, ws, 0 if ws is None else ws.numel()
+
+
+def layernorm_fwd(x: torch.Tensor, gamma=None, beta=None, eps: float = LN_EPS, act_slope: float = 1.0, p: float = 0.0,
+                  rng=None, residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None):
+    """``(y, mean, rstd)`` with ``y = dropout(act((x - mean) * rstd * gamma + beta)) (+ residual)``, the norm over the last
+    axis.  ``act_slope``: activation code (1 none, 0 ... 1 leaky slope, ACT_SILU, ACT_MISH); ``p`` / ``rng``: see
+    :func:`dropout`.  x float32, bfloat16 or float16 with evenly strided rows; gamma / beta float32 or x's type, either may
+    be None; mean / rstd are float32 of ``x.shape[:-1]``.  ``out`` may be ``x`` or ``residual``."""
+    d = _ln_desc(x, gamma, beta, eps, act_slope, p, rng)
+    if residual is not None:
+        d.ld_res = _row_operand(residual, "residual", x)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        d.ld_out = d.cols
+    else:
+        d.ld_out = _row_operand(out, "out", x)
+    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    check(L.load().fcd_layernorm_fwd(C.byref(d), x.data_ptr(), ptr(gamma), ptr(beta), ptr(residual), out.data_ptr(),
+                                     mean.data_ptr(), rstd.data_ptr(), stream()), "layernorm_fwd")
+    return out, mean, rstd
+
+
+def layernorm_bwd(gy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, gamma=None, beta=None,
+                  act_slope: float = 1.0, p: float = 0.0, rng=None, want_affine: bool = True, dgamma=None, dbeta=None,
+                  accumulate: bool = False, out: Optional[torch.Tensor] = None):
+    """``(dx, dgamma, dbeta)`` of :func:`layernorm_fwd` (the residual's gradient is ``gy`` itself); mask and activation
+    slope are recomputed.  ``dgamma`` / ``dbeta`` given: written (``accumulate``: added to) in place.  Bit-reproducible:
+    row sums run in a fixed order."""
+    d = _ln_desc(x, gamma, beta, 0.0, act_slope, p, rng)
+    d.ld_gy = _row_operand(gy, "gy", x)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        d.ld_out = d.cols
+    else:
+        d.ld_out = _row_operand(out, "out", x)
+    dgamma, dbeta, ws, wn = _ln_affine(gamma, beta, want_affine, dgamma, dbeta, accumulate, d, x)
+    check(L.load().fcd_layernorm_bwd(C.byref(d), gy.data_ptr(), x.data_ptr(), _ln_stat(mean, "mean", d, x),
+                                     _ln_stat(rstd, "rstd", d, x), ptr(gamma), ptr(beta), out.data_ptr(), ptr(dgamma),
+                                     ptr(dbeta), int(accumulate), ptr(ws), wn, stream()), "layernorm_bwd")
+    return out, dgamma, dbeta
+
+
+def layernorm_bwd2(ggx: torch.Tensor, gy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, gamma=None,
+                   beta=None, act_slope: float = 1.0, p: float = 0.0, rng=None, want_affine: bool = True, dgamma=None,
+                   dbeta=None, accumulate: bool = False):
+    """Backward of :func:`layernorm_bwd`'s ``dx`` for its cotangent ``ggx`` (what a gradient penalty needs):
+    ``(ggy, gx, dgamma, dbeta)``, the cotangents of ``gy`` and ``x`` and the parameters' gradients."""
+    d = _ln_desc(x, gamma, beta, 0.0, act_slope, p, rng)
+    d.ld_gy = _row_operand(gy, "gy", x)
+    d.ld_ggx = _row_operand(ggx, "ggx", x)
+    d.ld_out = d.ld_ggy = d.cols
+    ggy = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    gx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dgamma, dbeta, ws, wn = _ln_affine(gamma, beta, want_affine, dgamma, dbeta, accumulate, d, x)
+    check(L.load().fcd_layernorm_bwd2(C.byref(d), ggx.data_ptr(), gy.data_ptr(), x.data_ptr(), _ln_stat(mean, "mean", d, x),
+                                      _ln_stat(rstd, "rstd", d, x), ptr(gamma), ptr(beta), ggy.data_ptr(), gx.data_ptr(),
+                                      ptr(dgamma), ptr(dbeta), int(accumulate), ptr(ws), wn, stream()), "layernorm_bwd2")
+    return ggy, gx, dgamma, dbeta
 
 
 # --------------------------------------------------------------------------- #

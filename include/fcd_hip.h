@@ -474,6 +474,76 @@ int fcd_valid_minmax(const float* diff, const uint8_t* target, size_t n, float* 
 int fcd_threshold_hist(const float* diff, const uint8_t* target, size_t n, const float* thresholds, int T,
                        unsigned long long* hist, void* stream);
 
+/* ------------------------------------------------------------------------- *
+ * Layer norm over the last axis, with activation, dropout and residual fused, its backward and the backward of that
+ * backward; dropout by itself.  No reference counterpart: its critic has no norm and no dropout.  A WGAN-GP critic
+ * cannot take a norm that couples samples, and its gradient penalty differentiates the input gradient again.
+ *
+ * A tensor is `rows` rows of `cols` contiguous elements of type `dtype`, `ld_*` elements apart (ld >= cols for what is
+ * written; an input's may be anything >= 0, 0 repeats one row).  No alignment beyond the element's own is asked for.
+ * gamma / beta / dgamma / dbeta are vectors of `cols` elements of type `param_dtype` (FCD_DT_F32, or the same as
+ * `dtype`); mean / rstd are fp32 vectors of `rows`.  All sums are fp32, rounded to the element type once at the end.
+ * An output may be the same tensor (address and row stride) as an input of the element type; any other overlap between
+ * them is refused.
+ *
+ * Dropout: element i of the rows x cols matrix, i = row * cols + col, takes the 16 bits number i % 8 (low half of word 0
+ * first) of block offset + i / 8 of Philox4x32-10 keyed with `seed` (Salmon, Moraes, Dror, Shaw: "Parallel random
+ * numbers: as easy as 1, 2, 3", SC 2011) and is dropped where they are below t = round(65536 * drop_p); what stays is
+ * multiplied by 65536 / (65536 - t).  A dropped element is 0 whatever it held, NaN included.  The mask is recomputed
+ * wherever it is needed and never stored.  `rng` not NULL: {seed, offset} are read from these two device words instead
+ * (desc.offset is added to the second), so that a captured graph draws other masks at every replay.
+ * ------------------------------------------------------------------------- */
+#define FCD_DT_F32 0
+#define FCD_DT_BF16 1
+#define FCD_DT_F16 2
+
+typedef struct FcdLayerNormDesc {
+  int64_t rows, cols;
+  int64_t ld_x;             /* x                                                     */
+  int64_t ld_res;           /* residual (fwd)                                        */
+  int64_t ld_gy;            /* gy (bwd, bwd2)                                        */
+  int64_t ld_ggx;           /* ggx (bwd2)                                            */
+  int64_t ld_out;           /* y (fwd), dx (bwd), gx (bwd2)                          */
+  int64_t ld_ggy;           /* ggy (bwd2)                                            */
+  uint64_t seed, offset;    /* dropout; see above                                    */
+  const uint64_t* rng;      /* device, two words, 8-byte aligned; or NULL            */
+  double drop_p;            /* 0 .. 1; 0: no dropout                                 */
+  float eps;                /* added to the (biased) variance; fwd only              */
+  float act;                /* 0 .. 1: leaky slope (1 = none); FCD_ACT_SILU / _MISH  */
+  int32_t dtype;            /* FCD_DT_*: x, residual, gy, ggx, y, dx, ggy, gx        */
+  int32_t param_dtype;      /* FCD_DT_F32 or dtype                                   */
+} FcdLayerNormDesc;
+
+int fcd_layernorm_desc_bytes(void);
+/* y = drop(act((x - mean) * rstd * gamma + beta)) (+ residual).  gamma NULL: 1; beta NULL: 0; mean and rstd (outputs) may
+ * both be NULL. */
+int fcd_layernorm_fwd(const FcdLayerNormDesc* d, const void* x, const void* gamma, const void* beta,
+                      const void* residual, void* y, float* mean, float* rstd, void* stream);
+/* Scratch of fcd_layernorm_bwd / _bwd2 when they compute dgamma / dbeta (0 without them). */
+size_t fcd_layernorm_workspace_bytes(const FcdLayerNormDesc* d);
+/* With u = xhat * gamma + beta, g1 = drop(gy) * act'(u), a = g1 * gamma:
+ *   dx = rstd * (a - mean(a) - xhat * mean(a * xhat)),  dgamma (+)= sum_rows g1 * xhat,  dbeta (+)= sum_rows g1.
+ * (residual's gradient is gy itself.)  dgamma / dbeta NULL: not computed.  Row sums in a fixed order, no atomics. */
+int fcd_layernorm_bwd(const FcdLayerNormDesc* d, const void* gy, const void* x, const float* mean, const float* rstd,
+                      const void* gamma, const void* beta, void* dx, void* dgamma, void* dbeta, int accumulate,
+                      void* workspace, size_t workspace_bytes, void* stream);
+/* Backward of dx: ggx is the cotangent v of dx (dgamma's and dbeta's cotangents are taken as zero).
+ *   t = rstd * (v - mean(v) - xhat * mean(v xhat)),  q = drop(gy) * act''(u) * gamma * t,
+ *   ggy = drop(act'(u) * gamma * t),
+ *   h = q * gamma - rstd * (v * mean(a xhat) + a * mean(v xhat)),
+ *   gx = rstd * (h - mean(h) - xhat * mean(h xhat)) - rstd^2 * xhat * (mean(v a) - mean(v) mean(a) - mean(v xhat) mean(a xhat)),
+ *   dgamma (+)= sum_rows (g1 * t + q * xhat),  dbeta (+)= sum_rows q. */
+int fcd_layernorm_bwd2(const FcdLayerNormDesc* d, const void* ggx, const void* gy, const void* x, const float* mean,
+                       const float* rstd, const void* gamma, const void* beta, void* ggy, void* gx, void* dgamma,
+                       void* dbeta, int accumulate, void* workspace, size_t workspace_bytes, void* stream);
+/* y = drop(x) (+ residual); its own backward (x: the incoming gradient, same seed and offset). */
+int fcd_dropout(const void* x, const void* residual, void* y, int64_t rows, int64_t cols, int64_t ld_x, int64_t ld_res,
+                int64_t ld_y, int dtype, double drop_p, uint64_t seed, uint64_t offset, const uint64_t* rng,
+                void* stream);
+/* taken[0..1] = state[0..1], then state[1] += blocks (device words): hands out a range of blocks of the generator, also
+ * inside a captured graph.  Rows * cols elements use (rows * cols + 7) / 8 blocks. */
+int fcd_dropout_take(uint64_t* state, uint64_t* taken, uint64_t blocks, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
