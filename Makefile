@@ -3,7 +3,7 @@ HIPCC ?= /opt/rocm/bin/hipcc
 ARCH ?= gfx950
 SRCS := $(wildcard fcd_amd/csrc/*.hip)
 OBJS := $(SRCS:.hip=.o)
-HDRS := include/fcd_hip.h fcd_amd/csrc/fcd_common.h fcd_amd/csrc/fcd_rows.h
+HDRS := include/fcd_hip.h fcd_amd/csrc/fcd_common.h fcd_amd/csrc/fcd_rows.h fcd_amd/csrc/fcd_layernorm.h
 FLAGS := --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -Wall -Wno-unused-function
 # no packed fp32 instructions: some of their forms have given wrong results on these cards (the host pass does not know
 # the feature and says so; harmless)

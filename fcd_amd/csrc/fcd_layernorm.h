@@ -1,0 +1,232 @@
+// Shared by the layer norm's three directions (layernorm_fwd.hip, layernorm_bwd.hip, layernorm_bwd2.hip).
+#pragma once
+#include "fcd_rows.h"
+
+struct LnArgs {
+  const void *x, *res, *gy, *ggx, *gamma, *beta;
+  void *out, *ggy;
+  float *mean, *rstd;      // written by fwd, read by bwd / bwd2
+  float* partial;          // [groups][2][cols]: a workgroup's sums of dgamma and dbeta; or NULL
+  long rows, cols, ld_x, ld_res, ld_gy, ld_ggx, ld_out, ld_ggy;
+  float eps, act;
+  int param_f32;
+  Drop drop;
+};
+
+// layernorm.hip
+int ln_check(const char* who, const FcdLayerNormDesc* d, LnArgs* a);
+int ln_check_vectors(const char* who, const FcdLayerNormDesc* d, const void* gamma, const void* beta, const void* mean,
+                     const void* rstd);
+int ln_check_affine(const char* who, const FcdLayerNormDesc* d, const void* dgamma, const void* dbeta, void* workspace,
+                    size_t workspace_bytes, LnArgs* a);
+int ln_finish(const char* who, const FcdLayerNormDesc* d, const LnArgs& a, int groups, void* dgamma, void* dbeta, int accumulate,
+              hipStream_t st);
+int ln_groups(int64_t rows, int64_t cols);   // workgroups of the backward passes
+
+// Where a row lives.  Up to 1024 columns (G lanes of a wave, NV units of 8 elements a lane): the row is read once into
+// registers and its sums stay inside the wave, so a workgroup of 256 works on 256 / G rows with no barrier.  Up to 16384: G
+// threads, one workgroup per row, one barrier per sum.  Beyond: ln_*_long reads the row again from cache for every pass.
+#define LN_FOR_EACH_SHAPE(F) \
+  F(4, 1) F(8, 1) F(16, 1) F(32, 1) F(64, 1) F(64, 2) F(256, 1) F(256, 2) F(512, 2) F(1024, 2)
+
+struct LnShape {
+  int g, nv;   // g 0: the long form
+};
+
+static inline LnShape ln_shape(int64_t cols) {
+  const int64_t units = (cols + 7) / 8;
+#define PICK(G, NV) \
+  if (units <= (G) * (NV)) return {G, NV};
+  LN_FOR_EACH_SHAPE(PICK)
+#undef PICK
+  return {0, 0};
+}
+
+template <typename T>
+__device__ __forceinline__ void load_param(const void* p, int f32, long c, long n, float none, float (&v)[8]) {
+  if (!p) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = none;
+  } else if (f32) {
+    load8((const float*)p + c, n, v);
+  } else {
+    load8((const T*)p + c, n, v);
+  }
+}
+
+// 8 elements as they are in memory; the ones past n are 0
+template <typename T>
+__device__ __forceinline__ void load_raw(const T* p, long n, typename Oct<T>::type& o) {
+  if (n >= 8) {
+    o = *reinterpret_cast<const typename Oct<T>::type*>(p);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = j < n ? p[j] : (T)0.f;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void widen(const typename Oct<T>::type& o, float (&v)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = (float)o[j];
+}
+
+// ---------------------------------------------------------------- sums -----------------
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+
+// Sum over groups of G neighbouring lanes, in every lane: swaps inside quads, mirrors of 8 and 16 lanes (all lanes of a
+// smaller group already hold the same value there), then the row and half swaps of gfx950.  No LDS round trip.
+template <int G>
+__device__ __forceinline__ float lanes_sum(float v) {
+  if constexpr (G >= 2) v += dpp<0xB1>(v);
+  if constexpr (G >= 4) v += dpp<0x4E>(v);
+  if constexpr (G >= 8) v += dpp<0x141>(v);
+  if constexpr (G >= 16) v += dpp<0x140>(v);
+  if constexpr (G >= 32) {
+    const auto s = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+    const unsigned lo = s[0], hi = s[1];
+    v = __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+  }
+  if constexpr (G >= 64) {
+    const auto s = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+    const unsigned lo = s[0], hi = s[1];
+    v = __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+  }
+  return v;
+}
+
+// Sums of K values over the G threads of a row, in every thread.  More than a wave: one barrier; `turn` alternates between two
+// buffers, and a wave writes to one again only behind the barrier of the other, which every wave reaches after its reads.
+template <int G, int K>
+struct RowSums {
+  static constexpr int WAVES = G > 64 ? G / 64 : 1;
+  __device__ __forceinline__ static void run(float (&s)[K], float* sm, int& turn) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) s[k] = lanes_sum<(G < 64 ? G : 64)>(s[k]);
+    if constexpr (G > 64) {
+      float* buf = sm + turn * WAVES * K;
+      turn ^= 1;
+      const int w = threadIdx.x >> 6;
+      if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) buf[w * K + k] = s[k];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) t += buf[i * K + k];
+        s[k] = t;
+      }
+    }
+  }
+};
+
+// ---------------------------------------------------------------- activations ----------
+// The smooth ones from one hardware exponential and one hardware reciprocal (a step of fp32 each).  exp(u) as 2^(u log2 e)
+// loses |u| / 2 steps relative; what it is used in changes by at most |u| s (1 - s) < 0.23 times that.
+// mish, e = exp(u), n = e (e + 2): tanh(log(1 + e)) = n / (n + 2), its derivative w = 4 e (1 + e) / (n + 2)^2.
+__device__ __forceinline__ float fast_exp(float u) { return __builtin_amdgcn_exp2f(u * 1.44269504088896341f); }
+
+template <int ORDER>
+__device__ __forceinline__ float ln_act(float u, float code) {
+  if (code <= 1.f) {
+    const float s = u > 0.f ? 1.f : code;
+    return ORDER == 0 ? u * s : ORDER == 1 ? s : 0.f;
+  }
+  if (code == FCD_ACT_SILU) {
+    const float sg = __builtin_amdgcn_rcpf(1.f + fast_exp(-u));
+    if (ORDER == 0) return u * sg;
+    if (ORDER == 1) return sg * (1.f + u * (1.f - sg));
+    return sg * (1.f - sg) * (2.f + u * (1.f - 2.f * sg));
+  }
+  const float e = fast_exp(fminf(u, 20.f)), n = e * (e + 2.f), r = __builtin_amdgcn_rcpf(n + 2.f);
+  const float th = n * r;
+  if (ORDER == 0) return u * th;
+  const float w = 4.f * e * (1.f + e) * r * r;
+  if (ORDER == 1) return th + u * w;
+  const float sg = e * __builtin_amdgcn_rcpf(1.f + e);
+  return 2.f * w + u * w * ((1.f - sg) - 2.f * th * sg);
+}
+
+// ---------------------------------------------------------------- backward passes ------
+// Long rows: what the backward passes need of 8 elements, xhat, g1 = drop(gy) act'(u), a = g1 gamma; elements past the row's end: 0.
+struct Eight {
+  float xh[8], gy[8], u[8], ga[8], g1[8], a[8];
+  uint32_t keep;
+};
+
+template <typename T>
+__device__ __forceinline__ void load_eight(const LnArgs& p, long row, long c, float mean, float rstd, Eight& e) {
+  const long n = p.cols - c;
+  float be[8];
+  load8((const T*)p.x + row * p.ld_x + c, n, e.xh);
+  load8((const T*)p.gy + row * p.ld_gy + c, n, e.gy);
+  load_param<T>(p.gamma, p.param_f32, c, n, 1.f, e.ga);
+  load_param<T>(p.beta, p.param_f32, c, n, 0.f, be);
+  e.keep = 0xff;
+  if (p.drop.t) {
+    e.keep = drop_keep8(p.drop, (uint64_t)(row * p.cols + c));
+    drop_apply(p.drop, e.keep, e.gy);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    e.xh[j] = j < n ? (e.xh[j] - mean) * rstd : 0.f;
+    e.u[j] = e.xh[j] * e.ga[j] + be[j];
+    e.g1[j] = j < n ? e.gy[j] * ln_act<1>(e.u[j], p.act) : 0.f;
+    e.a[j] = e.g1[j] * e.ga[j];
+  }
+}
+
+// Adds to this workgroup's sums; a thread meets the same columns in every row, so nothing else touches them.
+__device__ __forceinline__ void add_partial(float* p, long n, bool first, const float (&v)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < n) p[j] = first ? v[j] : p[j] + v[j];
+}
+
+// Affine sums of a workgroup whose threads each kept NV * 8 columns in registers: over the groups of a wave by exchanges, over
+// the waves through LDS, in a fixed order; then to the workgroup's place in the scratch.
+template <int G, int NV>
+constexpr int affine_lds() { return G > 64 ? 1 : 4 * 2 * G * NV * 8; }
+
+template <int G, int NV>
+__device__ __forceinline__ void write_partial(const LnArgs& p, float (&dg)[NV][8], float (&db)[NV][8], float* sm) {
+  float* part = p.partial + (long)blockIdx.x * 2 * p.cols;
+  const int lane = threadIdx.x % G;
+  if constexpr (G > 64) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const long c = (lane + k * G) * 8, n = p.cols - c;
+      store8(part + c, n, dg[k]);
+      store8(part + p.cols + c, n, db[k]);
+    }
+  } else {
+    const int w = threadIdx.x >> 6;
+    constexpr int W = G * NV * 8;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float a = dg[k][j], b = db[k][j];
+#pragma unroll
+        for (int o = G; o < 64; o <<= 1) {
+          a += __shfl_xor(a, o, 64);
+          b += __shfl_xor(b, o, 64);
+        }
+        if ((threadIdx.x & 63) < G) {
+          sm[(w * 2 + 0) * W + (lane + k * G) * 8 + j] = a;
+          sm[(w * 2 + 1) * W + (lane + k * G) * 8 + j] = b;
+        }
+      }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * W; i += 256) {
+      const int which = i / W, c = i % W;
+      if (c < p.cols) part[which * p.cols + c] = (sm[i] + sm[2 * W + i]) + (sm[4 * W + i] + sm[6 * W + i]);
+    }
+  }
+}

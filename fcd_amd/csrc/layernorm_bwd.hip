@@ -1,0 +1,172 @@
+// Layer norm backward: dx, and the row sums of the affine gradients.
+#include "fcd_layernorm.h"
+
+namespace {
+
+// A row's x and gy in registers, one exchange for both of its sums, dx out; a thread meets the same columns in every row, so
+// the affine sums stay in its registers until the last row.  The next row's loads are in flight meanwhile.
+template <typename T, int G, int NV, bool EPI>
+__global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd_rows(LnArgs p) {
+  constexpr int TH = G > 64 ? G : 256, RPB = TH / G, WAVES = RowSums<G, 2>::WAVES;
+  __shared__ float sm[2 * 2 * WAVES];
+  __shared__ float aff[affine_lds<G, NV>()];
+  int turn = 0;
+  if (EPI) drop_state(p.drop);
+  const int lane = threadIdx.x % G;
+  const float inv = 1.f / (float)p.cols;
+  float ga[NV][8], be[NV][8], dg[NV][8], db[NV][8];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const long c = (lane + k * G) * 8;
+    load_param<T>(p.gamma, p.param_f32, c, p.cols - c, 1.f, ga[k]);
+    if (EPI) load_param<T>(p.beta, p.param_f32, c, p.cols - c, 0.f, be[k]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dg[k][j] = db[k][j] = 0.f;
+  }
+  typename Oct<T>::type nx[NV], ng[NV];
+  float nmean = 0.f, nrstd = 0.f;
+  long row = (long)blockIdx.x * RPB + threadIdx.x / G;
+  auto fetch = [&](long r) {
+    const bool here = r < p.rows;
+    nmean = here ? p.mean[r] : 0.f;
+    nrstd = here ? p.rstd[r] : 0.f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const long c = (lane + k * G) * 8, n = here ? p.cols - c : 0;
+      load_raw<T>((const T*)p.x + r * p.ld_x + c, n, nx[k]);
+      load_raw<T>((const T*)p.gy + r * p.ld_gy + c, n, ng[k]);
+    }
+  };
+  fetch(row);
+  // every thread makes the same number of turns: the sums need whole groups
+  const long step = (long)gridDim.x * RPB, turns = (p.rows - (long)blockIdx.x * RPB + step - 1) / step;
+  for (long it = 0; it < turns; ++it, row += step) {
+    const float mean = nmean, rstd = nrstd;
+    float xh[NV][8], a[NV][8];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      widen<T>(nx[k], xh[k]);
+      widen<T>(ng[k], a[k]);
+    }
+    if (it + 1 < turns) fetch(row + step);
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if (EPI && p.drop.t) drop_apply(p.drop, drop_keep8(p.drop, (uint64_t)(row * p.cols + (lane + k * G) * 8)), a[k]);
+      float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        xh[k][j] = (xh[k][j] - mean) * rstd;          // (absent elements: gy is 0, and so is all that follows)
+        float g1 = a[k][j];
+        if (EPI) g1 *= ln_act<1>(fmaf(xh[k][j], ga[k][j], be[k][j]), p.act);
+        dg[k][j] = fmaf(g1, xh[k][j], dg[k][j]);
+        db[k][j] += g1;
+        a[k][j] = g1 * ga[k][j];
+        s0 += a[k][j];
+        s1 = fmaf(a[k][j], xh[k][j], s1);
+      }
+      s[0] += s0;
+      s[1] += s1;
+    }
+    RowSums<G, 2>::run(s, sm, turn);
+    const float am = s[0] * inv, ax = s[1] * inv;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const long c = (lane + k * G) * 8, n = row < p.rows ? p.cols - c : 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a[k][j] = rstd * (a[k][j] - am - xh[k][j] * ax);
+      store8((T*)p.out + row * p.ld_out + c, n, a[k]);
+    }
+  }
+  if (p.partial) write_partial<G, NV>(p, dg, db, aff);
+}
+
+// Rows too long for registers: both operands read again for every pass, the affine sums kept in the scratch.
+template <typename T>
+__global__ __launch_bounds__(1024) void ln_bwd_long(LnArgs p) {
+  constexpr int TH = 1024;
+  __shared__ float sm[2 * 2 * TH / 64];
+  int turn = 0;
+  drop_state(p.drop);
+  const float inv = 1.f / (float)p.cols;
+  for (long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    const float mean = p.mean[row], rstd = p.rstd[row];
+    float s[2] = {0.f, 0.f};
+    for (long c = threadIdx.x * 8; c < p.cols; c += TH * 8) {
+      Eight e;
+      load_eight<T>(p, row, c, mean, rstd, e);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        s[0] += e.a[j];
+        s[1] += e.a[j] * e.xh[j];
+      }
+    }
+    RowSums<TH, 2>::run(s, sm, turn);
+    const float am = s[0] * inv, ax = s[1] * inv;
+    for (long c = threadIdx.x * 8; c < p.cols; c += TH * 8) {
+      const long n = p.cols - c;
+      Eight e;
+      load_eight<T>(p, row, c, mean, rstd, e);
+      float dx[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) dx[j] = rstd * (e.a[j] - am - e.xh[j] * ax);
+      if (p.partial) {
+        float* part = p.partial + (long)blockIdx.x * 2 * p.cols + c;
+        float dg[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) dg[j] = e.g1[j] * e.xh[j];
+        add_partial(part, n, row == blockIdx.x, dg);
+        add_partial(part + p.cols, n, row == blockIdx.x, e.g1);
+      }
+      store8((T*)p.out + row * p.ld_out + c, n, dx);
+    }
+  }
+}
+
+template <typename T>
+void launch(const LnArgs& a, int groups, hipStream_t st) {
+  const LnShape s = ln_shape(a.cols);
+  const bool epi = a.act != 1.f || a.drop.t;
+  if (s.g == 0) {
+    ln_bwd_long<T><<<groups, 1024, 0, st>>>(a);
+    return;
+  }
+#define SHAPE(G, NV)                                                                            \
+  if (s.g == G && s.nv == NV) {                                                                 \
+    if (epi) ln_bwd_rows<T, G, NV, true><<<groups, G > 64 ? G : 256, 0, st>>>(a);               \
+    else ln_bwd_rows<T, G, NV, false><<<groups, G > 64 ? G : 256, 0, st>>>(a);                  \
+  }
+  LN_FOR_EACH_SHAPE(SHAPE)
+#undef SHAPE
+}
+
+}  // namespace
+
+extern "C" int fcd_layernorm_bwd(const FcdLayerNormDesc* d, const void* gy, const void* x, const float* mean, const float* rstd,
+                                 const void* gamma, const void* beta, void* dx, void* dgamma, void* dbeta, int accumulate,
+                                 void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "fcd_layernorm_bwd";
+  LnArgs a;
+  FCD_TRY(ln_check(who, d, &a));
+  const int es = fcd_dt_bytes(d->dtype);
+  const RowView vx{"x", x, d->ld_x}, vg{"gy", gy, d->ld_gy}, vo{"dx", dx, d->ld_out};
+  FCD_TRY(fcd_check_rows(who, vx, d->rows, d->cols, es, false));
+  FCD_TRY(fcd_check_rows(who, vg, d->rows, d->cols, es, false));
+  FCD_TRY(fcd_check_rows(who, vo, d->rows, d->cols, es, true));
+  FCD_TRY(fcd_check_apart(who, vo, vx, d->rows, d->cols, es, true));
+  FCD_TRY(fcd_check_apart(who, vo, vg, d->rows, d->cols, es, true));
+  FCD_TRY(ln_check_vectors(who, d, gamma, beta, mean, rstd));
+  FCD_REQUIRE(d->rows == 0 || (mean && rstd), "%s: mean / rstd are NULL", who);
+  FCD_TRY(ln_check_affine(who, d, dgamma, dbeta, workspace, workspace_bytes, &a));
+  a.x = x, a.gy = gy, a.gamma = gamma, a.beta = beta, a.out = dx, a.mean = (float*)mean, a.rstd = (float*)rstd;
+  const int groups = ln_groups(d->rows, d->cols);
+  hipStream_t st = fcd_stream(stream);
+  if (d->rows) {
+    if (d->dtype == FCD_DT_F32) launch<float>(a, groups, st);
+    else if (d->dtype == FCD_DT_BF16) launch<bf16_t>(a, groups, st);
+    else launch<f16_t>(a, groups, st);
+    FCD_TRY(fcd_check_launch(who));
+  }
+  return dgamma || dbeta ? ln_finish(who, d, a, groups, dgamma, dbeta, accumulate, st) : FCD_OK;
+}
+

@@ -1,0 +1,240 @@
+// Layer norm: backward of the backward pass (the cotangents of gy and x for one of dx), for gradient penalties.
+#include "fcd_layernorm.h"
+
+namespace {
+
+// A row's x, gy and v = ggx in registers; five sums in one exchange, two more if the activation is curved.
+template <typename T, int G, int NV, bool EPI>
+__global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd2_rows(LnArgs p) {
+  constexpr int TH = G > 64 ? G : 256, RPB = TH / G, WAVES = RowSums<G, 5>::WAVES;
+  __shared__ float sm[2 * 5 * WAVES], sm2[2 * 2 * WAVES];
+  __shared__ float aff[affine_lds<G, NV>()];
+  int turn = 0, turn2 = 0;
+  if (EPI) drop_state(p.drop);
+  const int lane = threadIdx.x % G;
+  const float inv = 1.f / (float)p.cols;
+  const bool smooth = EPI && p.act > 1.f;
+  float ga[NV][8], be[NV][8], dg[NV][8], db[NV][8];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const long c = (lane + k * G) * 8;
+    load_param<T>(p.gamma, p.param_f32, c, p.cols - c, 1.f, ga[k]);
+    if (EPI) load_param<T>(p.beta, p.param_f32, c, p.cols - c, 0.f, be[k]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dg[k][j] = db[k][j] = 0.f;
+  }
+  // every thread makes the same number of turns: the sums need whole groups
+  const long step = (long)gridDim.x * RPB, turns = (p.rows - (long)blockIdx.x * RPB + step - 1) / step;
+  long row = (long)blockIdx.x * RPB + threadIdx.x / G;
+  for (long it = 0; it < turns; ++it, row += step) {
+    const bool here = row < p.rows;
+    const float mean = here ? p.mean[row] : 0.f, rstd = here ? p.rstd[row] : 0.f;
+    typename Oct<T>::type rx[NV], rg[NV], rv[NV];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const long c = (lane + k * G) * 8, n = here ? p.cols - c : 0;
+      load_raw<T>((const T*)p.x + row * p.ld_x + c, n, rx[k]);
+      load_raw<T>((const T*)p.gy + row * p.ld_gy + c, n, rg[k]);
+      load_raw<T>((const T*)p.ggx + row * p.ld_ggx + c, n, rv[k]);
+    }
+    // xhat, drop(gy), v, and with an epilogue act'(u) and act''(u)
+    float xh[NV][8], g[NV][8], v[NV][8], d1[NV][8], q[NV][8], s[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
+    uint32_t keep[NV];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      widen<T>(rx[k], xh[k]);
+      widen<T>(rg[k], g[k]);
+      widen<T>(rv[k], v[k]);
+      keep[k] = 0xff;
+      if (EPI && p.drop.t) {
+        keep[k] = drop_keep8(p.drop, (uint64_t)(row * p.cols + (lane + k * G) * 8));
+        drop_apply(p.drop, keep[k], g[k]);
+      }
+      float t[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        xh[k][j] = (xh[k][j] - mean) * rstd;          // (absent elements: gy and v are 0, and so are their products)
+        if (EPI) {
+          const float u = fmaf(xh[k][j], ga[k][j], be[k][j]);
+          d1[k][j] = ln_act<1>(u, p.act);
+          q[k][j] = smooth ? ln_act<2>(u, p.act) : 0.f;
+        }
+        const float a = (EPI ? g[k][j] * d1[k][j] : g[k][j]) * ga[k][j];
+        t[0] += a;
+        t[1] = fmaf(a, xh[k][j], t[1]);
+        t[2] += v[k][j];
+        t[3] = fmaf(v[k][j], xh[k][j], t[3]);
+        t[4] = fmaf(v[k][j], a, t[4]);
+      }
+#pragma unroll
+      for (int i = 0; i < 5; ++i) s[i] += t[i];
+    }
+    RowSums<G, 5>::run(s, sm, turn);
+    const float am = s[0] * inv, ax = s[1] * inv, vm = s[2] * inv, vx = s[3] * inv;
+    const float sv = s[4] * inv - vm * am - vx * ax;
+    float q2[2] = {0.f, 0.f};
+    if (smooth) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        float q0 = 0.f, q1 = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          q[k][j] *= g[k][j] * ga[k][j] * (rstd * (v[k][j] - vm - xh[k][j] * vx));
+          const float qg = q[k][j] * ga[k][j];
+          q0 += qg;
+          q1 = fmaf(qg, xh[k][j], q1);
+        }
+        q2[0] += q0;
+        q2[1] += q1;
+      }
+      RowSums<G, 2>::run(q2, sm2, turn2);
+    }
+    const float hm = q2[0] * inv - rstd * (vm * ax + am * vx), hx = q2[1] * inv - 2.f * rstd * vx * ax;
+    const float srr = sv * rstd * rstd;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const long c = (lane + k * G) * 8, n = here ? p.cols - c : 0;
+      float gg[8], gx[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float t = rstd * (v[k][j] - vm - xh[k][j] * vx);
+        const float g1 = EPI ? g[k][j] * d1[k][j] : g[k][j];
+        const float qj = EPI ? q[k][j] : 0.f;
+        gg[j] = (EPI ? d1[k][j] * ga[k][j] : ga[k][j]) * t;
+        const float h = qj * ga[k][j] - rstd * (v[k][j] * ax + g1 * ga[k][j] * vx);
+        gx[j] = rstd * (h - hm - xh[k][j] * hx) - srr * xh[k][j];
+        dg[k][j] += g1 * t + qj * xh[k][j];           // (absent elements: g1 and q are 0)
+        db[k][j] += qj;
+      }
+      if (EPI && p.drop.t) drop_apply(p.drop, keep[k], gg);
+      store8((T*)p.ggy + row * p.ld_ggy + c, n, gg);
+      store8((T*)p.out + row * p.ld_out + c, n, gx);
+    }
+  }
+  if (p.partial) write_partial<G, NV>(p, dg, db, aff);
+}
+
+// Rows too long for registers: both operands read again for every pass, the affine sums kept in the scratch.
+template <typename T>
+__global__ __launch_bounds__(1024) void ln_bwd2_long(LnArgs p) {
+  constexpr int TH = 1024;
+  __shared__ float sm[2 * 5 * TH / 64];
+  int turn = 0, turn2 = 0;
+  __shared__ float sm2[2 * 2 * TH / 64];
+  drop_state(p.drop);
+  const float inv = 1.f / (float)p.cols;
+  const bool smooth = p.act > 1.f;
+  for (long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    const float mean = p.mean[row], rstd = p.rstd[row];
+    float s[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
+    for (long c = threadIdx.x * 8; c < p.cols; c += TH * 8) {
+      Eight e;
+      float v[8];
+      load_eight<T>(p, row, c, mean, rstd, e);
+      load8((const T*)p.ggx + row * p.ld_ggx + c, p.cols - c, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        s[0] += e.a[j];
+        s[1] += e.a[j] * e.xh[j];
+        s[2] += v[j];
+        s[3] += v[j] * e.xh[j];
+        s[4] += v[j] * e.a[j];
+      }
+    }
+    RowSums<TH, 5>::run(s, sm, turn);
+    const float am = s[0] * inv, ax = s[1] * inv, vm = s[2] * inv, vx = s[3] * inv;
+    const float sv = s[4] * inv - vm * am - vx * ax;
+    float q2[2] = {0.f, 0.f};
+    if (smooth) {
+      for (long c = threadIdx.x * 8; c < p.cols; c += TH * 8) {
+        Eight e;
+        float v[8];
+        load_eight<T>(p, row, c, mean, rstd, e);
+        load8((const T*)p.ggx + row * p.ld_ggx + c, p.cols - c, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float t = rstd * (v[j] - vm - e.xh[j] * vx);
+          const float qg = j < p.cols - c ? e.gy[j] * ln_act<2>(e.u[j], p.act) * e.ga[j] * t * e.ga[j] : 0.f;
+          q2[0] += qg;
+          q2[1] += qg * e.xh[j];
+        }
+      }
+      RowSums<TH, 2>::run(q2, sm2, turn2);
+    }
+    const float hm = q2[0] * inv - rstd * (vm * ax + am * vx), hx = q2[1] * inv - 2.f * rstd * vx * ax;
+    for (long c = threadIdx.x * 8; c < p.cols; c += TH * 8) {
+      const long n = p.cols - c;
+      Eight e;
+      float v[8], gg[8], gx[8], dg[8], q[8];
+      load_eight<T>(p, row, c, mean, rstd, e);
+      load8((const T*)p.ggx + row * p.ld_ggx + c, n, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float t = rstd * (v[j] - vm - e.xh[j] * vx);
+        q[j] = smooth ? e.gy[j] * ln_act<2>(e.u[j], p.act) * e.ga[j] * t : 0.f;
+        gg[j] = ln_act<1>(e.u[j], p.act) * e.ga[j] * t;
+        const float h = q[j] * e.ga[j] - rstd * (v[j] * ax + e.a[j] * vx);
+        gx[j] = rstd * (h - hm - e.xh[j] * hx) - sv * rstd * rstd * e.xh[j];
+        dg[j] = e.g1[j] * t + q[j] * e.xh[j];
+      }
+      if (p.drop.t) drop_apply(p.drop, e.keep, gg);
+      if (p.partial) {
+        float* part = p.partial + (long)blockIdx.x * 2 * p.cols + c;
+        add_partial(part, n, row == blockIdx.x, dg);
+        add_partial(part + p.cols, n, row == blockIdx.x, q);
+      }
+      store8((T*)p.ggy + row * p.ld_ggy + c, n, gg);
+      store8((T*)p.out + row * p.ld_out + c, n, gx);
+    }
+  }
+}
+
+template <typename T>
+void launch(const LnArgs& a, int groups, hipStream_t st) {
+  const LnShape s = ln_shape(a.cols);
+  const bool epi = a.act != 1.f || a.drop.t;
+  if (s.g == 0) {
+    ln_bwd2_long<T><<<groups, 1024, 0, st>>>(a);
+    return;
+  }
+#define SHAPE(G, NV)                                                                            \
+  if (s.g == G && s.nv == NV) {                                                                 \
+    if (epi) ln_bwd2_rows<T, G, NV, true><<<groups, G > 64 ? G : 256, 0, st>>>(a);              \
+    else ln_bwd2_rows<T, G, NV, false><<<groups, G > 64 ? G : 256, 0, st>>>(a);                 \
+  }
+  LN_FOR_EACH_SHAPE(SHAPE)
+#undef SHAPE
+}
+
+}  // namespace
+
+extern "C" int fcd_layernorm_bwd2(const FcdLayerNormDesc* d, const void* ggx, const void* gy, const void* x, const float* mean,
+                                  const float* rstd, const void* gamma, const void* beta, void* ggy, void* gx, void* dgamma,
+                                  void* dbeta, int accumulate, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "fcd_layernorm_bwd2";
+  LnArgs a;
+  FCD_TRY(ln_check(who, d, &a));
+  const int es = fcd_dt_bytes(d->dtype);
+  const RowView in[3] = {{"x", x, d->ld_x}, {"gy", gy, d->ld_gy}, {"ggx", ggx, d->ld_ggx}};
+  const RowView out[2] = {{"gx", gx, d->ld_out}, {"ggy", ggy, d->ld_ggy}};
+  for (const RowView& v : in) FCD_TRY(fcd_check_rows(who, v, d->rows, d->cols, es, false));
+  for (const RowView& v : out) {
+    FCD_TRY(fcd_check_rows(who, v, d->rows, d->cols, es, true));
+    for (const RowView& w : in) FCD_TRY(fcd_check_apart(who, v, w, d->rows, d->cols, es, true));
+  }
+  FCD_TRY(fcd_check_apart(who, out[0], out[1], d->rows, d->cols, es, false));
+  FCD_TRY(ln_check_vectors(who, d, gamma, beta, mean, rstd));
+  FCD_REQUIRE(d->rows == 0 || (mean && rstd), "%s: mean / rstd are NULL", who);
+  FCD_TRY(ln_check_affine(who, d, dgamma, dbeta, workspace, workspace_bytes, &a));
+  a.x = x, a.gy = gy, a.ggx = ggx, a.gamma = gamma, a.beta = beta, a.out = gx, a.ggy = ggy;
+  a.mean = (float*)mean, a.rstd = (float*)rstd;
+  const int groups = ln_groups(d->rows, d->cols);
+  hipStream_t st = fcd_stream(stream);
+  if (d->rows) {
+    if (d->dtype == FCD_DT_F32) launch<float>(a, groups, st);
+    else if (d->dtype == FCD_DT_BF16) launch<bf16_t>(a, groups, st);
+    else launch<f16_t>(a, groups, st);
+    FCD_TRY(fcd_check_launch(who));
+  }
+  return dgamma || dbeta ? ln_finish(who, d, a, groups, dgamma, dbeta, accumulate, st) : FCD_OK;
+}
