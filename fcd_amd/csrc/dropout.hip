@@ -4,23 +4,31 @@
 
 namespace {
 
+// 8 elements a thread and turn: x and the residual in, y out, one generator block between.  A workgroup stays in one row
+// (blockIdx.y and further rows below it); a tensor without gaps is one long row.
 template <typename T>
 __global__ __launch_bounds__(256) void dropout_kernel(const T* x, const T* res, T* y, long rows, long cols, long ld_x,
                                                       long ld_res, long ld_y, Drop d) {
   drop_state(d);
-  const long per_row = (cols + 7) / 8, total = rows * per_row;
-  for (long k = (long)blockIdx.x * 256 + threadIdx.x; k < total; k += (long)gridDim.x * 256) {
-    const long row = k / per_row, c = (k - row * per_row) * 8, n = cols - c;
-    float v[8];
-    load8(x + row * ld_x + c, n, v);
-    if (d.t) drop_apply(d, drop_keep8(d, (uint64_t)(row * cols + c)), v);
-    if (res) {
-      float r[8];
-      load8(res + row * ld_res + c, n, r);
+  for (long row = blockIdx.y; row < rows; row += gridDim.y) {
+    const T *xr = x + row * ld_x, *rr = res + row * ld_res;
+    T* yr = y + row * ld_y;
+    for (long c = ((long)blockIdx.x * 256 + threadIdx.x) * 8; c < cols; c += (long)gridDim.x * 256 * 8) {
+      const long n = cols - c;
+      float v[8], r[8];
+      load8(xr + c, n, v);
+      if (res) load8(rr + c, n, r);
+      if (d.t) {
+        uint32_t w[4];
+        drop_draw8(d, (uint64_t)(row * cols + c), w);
+        drop_apply(d, w, v);
+      }
+      if (res) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] += r[j];
+        for (int j = 0; j < 8; ++j) v[j] += r[j];
+      }
+      store8(yr + c, n, v);
     }
-    store8(y + row * ld_y + c, n, v);
   }
 }
 
@@ -54,9 +62,8 @@ extern "C" int fcd_dropout(const void* x, const void* residual, void* y, int64_t
     cols *= rows;
     rows = 1;
   }
-  const int64_t units = rows * ((cols + 7) / 8);
-  const int64_t blocks = (units + 255) / 256;
-  const dim3 grid((unsigned)(blocks < (1 << 20) ? blocks : (1 << 20)));
+  const int64_t bx = (cols + 2047) / 2048;
+  const dim3 grid((unsigned)(bx < (1 << 20) ? bx : (1 << 20)), (unsigned)(rows < 32768 ? rows : 32768));
   hipStream_t st = fcd_stream(stream);
 #define LAUNCH(T)                                                                                                     \
   dropout_kernel<T><<<grid, 256, 0, st>>>((const T*)x, (const T*)residual, (T*)y, rows, cols, ld_x, ld_res, ld_y, d)

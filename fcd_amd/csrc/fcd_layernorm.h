@@ -23,27 +23,38 @@ int ln_finish(const char* who, const FcdLayerNormDesc* d, const LnArgs& a, int g
               hipStream_t st);
 int ln_groups(int64_t rows, int64_t cols);   // workgroups of the backward passes
 
-// Where a row lives.  Up to 1024 columns (G lanes of a wave, NV units of 8 elements a lane): the row is read once into
-// registers and its sums stay inside the wave, so a workgroup of 256 works on 256 / G rows with no barrier.  Up to 16384: G
-// threads, one workgroup per row, one barrier per sum.  Beyond: ln_*_long reads the row again from cache for every pass.
-#define LN_FOR_EACH_SHAPE(F) \
+// Where a row lives: G threads with NV units of 8 elements each.  G <= 64: the row's sums stay inside a wave, and a workgroup
+// of 256 works on 256 / G rows with no barrier; G > 64: one workgroup per row, one barrier per sum.  Longer rows than the last
+// shape takes are read again from cache for every pass (ln_*_long).  The forward pass keeps two units a thread (fewer waves
+// meet at the barrier); the backward passes hold the affine sums as well and keep one.
+#define LN_FWD_SHAPES(F) \
   F(4, 1) F(8, 1) F(16, 1) F(32, 1) F(64, 1) F(64, 2) F(256, 1) F(256, 2) F(512, 2) F(1024, 2)
+#define LN_BWD_SHAPES(F) \
+  F(4, 1) F(8, 1) F(16, 1) F(32, 1) F(64, 1) F(128, 1) F(256, 1) F(512, 1) F(1024, 1)
 
 struct LnShape {
   int g, nv;   // g 0: the long form
 };
 
-static inline LnShape ln_shape(int64_t cols) {
+static inline LnShape ln_bwd_shape(int64_t cols) {
   const int64_t units = (cols + 7) / 8;
 #define PICK(G, NV) \
   if (units <= (G) * (NV)) return {G, NV};
-  LN_FOR_EACH_SHAPE(PICK)
+  LN_BWD_SHAPES(PICK)
 #undef PICK
   return {0, 0};
 }
 
-template <typename T>
-__device__ __forceinline__ void load_param(const void* p, int f32, long c, long n, float none, float (&v)[8]) {
+// The row of a thread (wave-uniform where it can be, so that row addresses live in scalar registers) and its first column.
+template <int G, int TH>
+__device__ __forceinline__ long first_row() {
+  if constexpr (G == TH) return blockIdx.x;
+  if constexpr (G == 64) return (long)blockIdx.x * (TH / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  return (long)blockIdx.x * (TH / G) + threadIdx.x / G;
+}
+
+template <typename T, typename N>
+__device__ __forceinline__ void load_param(const void* p, int f32, N c, N n, float none, float (&v)[8]) {
   if (!p) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = none;
@@ -55,8 +66,8 @@ __device__ __forceinline__ void load_param(const void* p, int f32, long c, long 
 }
 
 // 8 elements as they are in memory; the ones past n are 0
-template <typename T>
-__device__ __forceinline__ void load_raw(const T* p, long n, typename Oct<T>::type& o) {
+template <typename T, typename N>
+__device__ __forceinline__ void load_raw(const T* p, N n, typename Oct<T>::type& o) {
   if (n >= 8) {
     o = *reinterpret_cast<const typename Oct<T>::type*>(p);
   } else {
@@ -116,12 +127,7 @@ struct RowSums {
       }
       __syncthreads();
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        float t = 0.f;
-#pragma unroll
-        for (int i = 0; i < WAVES; ++i) t += buf[i * K + k];
-        s[k] = t;
-      }
+      for (int k = 0; k < K; ++k) s[k] = lanes_sum<WAVES>(buf[(threadIdx.x & (WAVES - 1)) * K + k]);
     }
   }
 };
@@ -132,52 +138,68 @@ struct RowSums {
 // mish, e = exp(u), n = e (e + 2): tanh(log(1 + e)) = n / (n + 2), its derivative w = 4 e (1 + e) / (n + 2)^2.
 __device__ __forceinline__ float fast_exp(float u) { return __builtin_amdgcn_exp2f(u * 1.44269504088896341f); }
 
-template <int ORDER>
-__device__ __forceinline__ float ln_act(float u, float code) {
+// The activation (d0) of 8 values, or its first (d1) and second (d2) derivative; what is NULL is not computed.
+__device__ __forceinline__ void ln_act8(const float (&u)[8], float code, float* d0, float* d1, float* d2) {
   if (code <= 1.f) {
-    const float s = u > 0.f ? 1.f : code;
-    return ORDER == 0 ? u * s : ORDER == 1 ? s : 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float s = u[j] > 0.f ? 1.f : code;
+      if (d0) d0[j] = u[j] * s;
+      if (d1) d1[j] = s;
+      if (d2) d2[j] = 0.f;
+    }
+  } else if (code == FCD_ACT_SILU) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float sg = __builtin_amdgcn_rcpf(1.f + fast_exp(-u[j])), ns = 1.f - sg;
+      if (d0) d0[j] = u[j] * sg;
+      if (d1) d1[j] = fmaf(u[j] * sg, ns, sg);
+      if (d2) d2[j] = sg * ns * fmaf(u[j], ns - sg, 2.f);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float e = fast_exp(fminf(u[j], 20.f)), n = e * (e + 2.f), r = __builtin_amdgcn_rcpf(n + 2.f), th = n * r;
+      if (d0) d0[j] = u[j] * th;
+      const float w = 4.f * e * (1.f + e) * r * r;
+      if (d1) d1[j] = fmaf(u[j], w, th);
+      if (d2) {
+        const float sg = e * __builtin_amdgcn_rcpf(1.f + e);
+        d2[j] = w * fmaf(u[j], (1.f - sg) - 2.f * th * sg, 2.f);
+      }
+    }
   }
-  if (code == FCD_ACT_SILU) {
-    const float sg = __builtin_amdgcn_rcpf(1.f + fast_exp(-u));
-    if (ORDER == 0) return u * sg;
-    if (ORDER == 1) return sg * (1.f + u * (1.f - sg));
-    return sg * (1.f - sg) * (2.f + u * (1.f - 2.f * sg));
-  }
-  const float e = fast_exp(fminf(u, 20.f)), n = e * (e + 2.f), r = __builtin_amdgcn_rcpf(n + 2.f);
-  const float th = n * r;
-  if (ORDER == 0) return u * th;
-  const float w = 4.f * e * (1.f + e) * r * r;
-  if (ORDER == 1) return th + u * w;
-  const float sg = e * __builtin_amdgcn_rcpf(1.f + e);
-  return 2.f * w + u * w * ((1.f - sg) - 2.f * th * sg);
 }
 
 // ---------------------------------------------------------------- backward passes ------
-// Long rows: what the backward passes need of 8 elements, xhat, g1 = drop(gy) act'(u), a = g1 gamma; elements past the row's end: 0.
+// Long rows: what the backward passes need of 8 elements: xhat, drop(gy), g1 = drop(gy) act'(u), a = g1 gamma; elements past
+// the row's end: 0.
 struct Eight {
-  float xh[8], gy[8], u[8], ga[8], g1[8], a[8];
-  uint32_t keep;
+  float xh[8], gy[8], ga[8], g1[8], a[8], d1[8], d2[8];
+  uint32_t w[4];
 };
 
-template <typename T>
+template <typename T, bool SECOND>
 __device__ __forceinline__ void load_eight(const LnArgs& p, long row, long c, float mean, float rstd, Eight& e) {
   const long n = p.cols - c;
-  float be[8];
+  float be[8], u[8];
   load8((const T*)p.x + row * p.ld_x + c, n, e.xh);
   load8((const T*)p.gy + row * p.ld_gy + c, n, e.gy);
   load_param<T>(p.gamma, p.param_f32, c, n, 1.f, e.ga);
   load_param<T>(p.beta, p.param_f32, c, n, 0.f, be);
-  e.keep = 0xff;
   if (p.drop.t) {
-    e.keep = drop_keep8(p.drop, (uint64_t)(row * p.cols + c));
-    drop_apply(p.drop, e.keep, e.gy);
+    drop_draw8(p.drop, (uint64_t)(row * p.cols + c), e.w);
+    drop_apply(p.drop, e.w, e.gy);
   }
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     e.xh[j] = j < n ? (e.xh[j] - mean) * rstd : 0.f;
-    e.u[j] = e.xh[j] * e.ga[j] + be[j];
-    e.g1[j] = j < n ? e.gy[j] * ln_act<1>(e.u[j], p.act) : 0.f;
+    u[j] = fmaf(e.xh[j], e.ga[j], be[j]);
+  }
+  ln_act8(u, p.act, nullptr, e.d1, SECOND ? e.d2 : nullptr);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    e.g1[j] = j < n ? e.gy[j] * e.d1[j] : 0.f;
     e.a[j] = e.g1[j] * e.ga[j];
   }
 }
@@ -197,13 +219,13 @@ constexpr int affine_lds() { return G > 64 ? 1 : 4 * 2 * G * NV * 8; }
 template <int G, int NV>
 __device__ __forceinline__ void write_partial(const LnArgs& p, float (&dg)[NV][8], float (&db)[NV][8], float* sm) {
   float* part = p.partial + (long)blockIdx.x * 2 * p.cols;
-  const int lane = threadIdx.x % G;
+  const int lane = threadIdx.x % G, cols = (int)p.cols;
   if constexpr (G > 64) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const long c = (lane + k * G) * 8, n = p.cols - c;
-      store8(part + c, n, dg[k]);
-      store8(part + p.cols + c, n, db[k]);
+      const int c = (lane + k * G) * 8;
+      store8(part + c, cols - c, dg[k]);
+      store8(part + cols + c, cols - c, db[k]);
     }
   } else {
     const int w = threadIdx.x >> 6;
@@ -226,7 +248,7 @@ __device__ __forceinline__ void write_partial(const LnArgs& p, float (&dg)[NV][8
     __syncthreads();
     for (int i = threadIdx.x; i < 2 * W; i += 256) {
       const int which = i / W, c = i % W;
-      if (c < p.cols) part[which * p.cols + c] = (sm[i] + sm[2 * W + i]) + (sm[4 * W + i] + sm[6 * W + i]);
+      if (c < cols) part[which * cols + c] = (sm[i] + sm[2 * W + i]) + (sm[4 * W + i] + sm[6 * W + i]);
     }
   }
 }

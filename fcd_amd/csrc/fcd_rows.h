@@ -14,8 +14,8 @@ template <> struct Oct<bf16_t> { typedef bf16_t type __attribute__((ext_vector_t
 template <> struct Oct<f16_t> { typedef f16_t type __attribute__((ext_vector_type(8), aligned(2))); };
 
 // n: how many of the 8 exist; the others read as 0 and are not written
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, long n, float (&v)[8]) {
+template <typename T, typename N>
+__device__ __forceinline__ void load8(const T* p, N n, float (&v)[8]) {
   if (n >= 8) {
     const typename Oct<T>::type o = *reinterpret_cast<const typename Oct<T>::type*>(p);
 #pragma unroll
@@ -26,8 +26,8 @@ __device__ __forceinline__ void load8(const T* p, long n, float (&v)[8]) {
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void store8(T* p, long n, const float (&v)[8]) {
+template <typename T, typename N>
+__device__ __forceinline__ void store8(T* p, N n, const float (&v)[8]) {
   if (n >= 8) {
     typename Oct<T>::type o;
 #pragma unroll
@@ -46,7 +46,10 @@ struct Drop {
   const uint64_t* rng;   // device words {seed, offset} in place of seed, added to offset; or NULL
   float scale;           // 65536 / (65536 - t); 0 if everything is dropped
   uint32_t t;            // dropped where the 16 bits are below t; 0: no dropout
+  uint32_t below;        // (t << 16) - 1
 };
+
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) { return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96); }
 
 // seed and first block, read once per thread
 __device__ __forceinline__ void drop_state(Drop& d) {
@@ -56,42 +59,52 @@ __device__ __forceinline__ void drop_state(Drop& d) {
   }
 }
 
-// Keep bits (bit j: element j stays) of one block of Philox4x32-10.
-__device__ __forceinline__ uint32_t drop_block(const Drop& d, uint64_t block) {
+// One block of Philox4x32-10.  (A product's two halves come from one 32 x 32 -> 64 bit multiply-add; three-way xors are
+// single instructions of gfx950.)
+__device__ __forceinline__ void drop_block(const Drop& d, uint64_t block, uint32_t (&w)[4]) {
   uint32_t c0 = (uint32_t)block, c1 = (uint32_t)(block >> 32), c2 = 0, c3 = 0;
   uint32_t k0 = (uint32_t)d.seed, k1 = (uint32_t)(d.seed >> 32);
 #pragma unroll
   for (int i = 0; i < 10; ++i) {
     const uint64_t p0 = (uint64_t)0xD2511F53u * c0, p1 = (uint64_t)0xCD9E8D57u * c2;
-    c0 = (uint32_t)(p1 >> 32) ^ c1 ^ k0;
+    c0 = xor3((uint32_t)(p1 >> 32), c1, k0);
     c1 = (uint32_t)p1;
-    c2 = (uint32_t)(p0 >> 32) ^ c3 ^ k1;
+    c2 = xor3((uint32_t)(p0 >> 32), c3, k1);
     c3 = (uint32_t)p0;
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
   }
-  const uint32_t w[4] = {c0, c1, c2, c3};
-  uint32_t m = 0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    m |= ((w[j] & 0xffffu) >= d.t ? 1u : 0u) << (2 * j);
-    m |= ((w[j] >> 16) >= d.t ? 2u : 0u) << (2 * j);
-  }
-  return m;
+  w[0] = c0, w[1] = c1, w[2] = c2, w[3] = c3;
 }
 
-// Keep bits of the elements i ... i + 7 of the matrix: one block if i is a multiple of 8, else the ends of two.
-__device__ __forceinline__ uint32_t drop_keep8(const Drop& d, uint64_t i) {
+// The eight 16-bit draws of the elements i ... i + 7 of the matrix: one block if i is a multiple of 8, else the end of one and
+// the beginning of the next.
+__device__ __forceinline__ void drop_draw8(const Drop& d, uint64_t i, uint32_t (&w)[4]) {
   const uint64_t block = d.offset + (i >> 3);
   const uint32_t phase = (uint32_t)i & 7u;
-  uint32_t m = drop_block(d, block);
-  if (phase) m = (m | drop_block(d, block + 1) << 8) >> phase;
-  return m;
+  drop_block(d, block, w);
+  if (phase) {
+    uint32_t n[4];
+    drop_block(d, block + 1, n);
+    // the two blocks as eight words, moved down by `phase` halves (scalars: an array would be indexed in memory)
+    const bool m4 = phase & 4u, m2 = phase & 2u, m1 = phase & 1u;
+    uint32_t a0 = m4 ? w[2] : w[0], a1 = m4 ? w[3] : w[1], a2 = m4 ? n[0] : w[2], a3 = m4 ? n[1] : w[3];
+    uint32_t a4 = m4 ? n[2] : n[0], a5 = m4 ? n[3] : n[1];
+    a0 = m2 ? a1 : a0, a1 = m2 ? a2 : a1, a2 = m2 ? a3 : a2, a3 = m2 ? a4 : a3, a4 = m2 ? a5 : a4;
+    w[0] = m1 ? a0 >> 16 | a1 << 16 : a0;
+    w[1] = m1 ? a1 >> 16 | a2 << 16 : a1;
+    w[2] = m1 ? a2 >> 16 | a3 << 16 : a2;
+    w[3] = m1 ? a3 >> 16 | a4 << 16 : a3;
+  }
 }
 
-__device__ __forceinline__ void drop_apply(const Drop& d, uint32_t keep, float (&v)[8]) {
+// A draw stays where it is at least t.  Both halves are compared in the upper 16 bits of a word, with (t << 16) - 1.
+__device__ __forceinline__ void drop_apply(const Drop& d, const uint32_t (&w)[4], float (&v)[8]) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = (keep >> j) & 1u ? v[j] * d.scale : 0.f;
+  for (int j = 0; j < 4; ++j) {
+    v[2 * j] = w[j] << 16 > d.below ? v[2 * j] * d.scale : 0.f;
+    v[2 * j + 1] = w[j] > d.below ? v[2 * j + 1] * d.scale : 0.f;
+  }
 }
 
 // ---------------------------------------------------------------- host checks ----------
@@ -101,6 +114,7 @@ static inline int fcd_make_drop(const char* who, double p, uint64_t seed, uint64
   FCD_REQUIRE(p >= 0.0 && p <= 1.0, "%s: the dropout probability must be in [0, 1]", who);
   FCD_REQUIRE(((uintptr_t)rng & 7u) == 0, "%s: rng must be 8-byte aligned", who);
   out->t = (uint32_t)__builtin_rint(p * 65536.0);
+  out->below = (uint32_t)(((uint64_t)out->t << 16) - 1);
   out->scale = out->t < 65536u ? (float)(65536.0 / (65536.0 - out->t)) : 0.f;
   out->seed = rng ? 0 : seed;
   out->offset = offset;

@@ -35,10 +35,16 @@ int reduce(const char* who, const LnArgs& a, int groups, void* dgamma, void* dbe
 
 }  // namespace
 
+#ifdef LN_TUNE
+#include <stdlib.h>
+static int64_t tune(const char* n, int64_t v) { const char* e = getenv(n); return e ? atoi(e) : v; }
+#else
+#define tune(n, v) (v)
+#endif
 int ln_groups(int64_t rows, int64_t cols) {
-  const LnShape s = ln_shape(cols);
+  const LnShape s = ln_bwd_shape(cols);
   const int64_t rpb = s.g > 0 && s.g <= 64 ? 256 / s.g : 1, need = (rows + rpb - 1) / rpb;
-  const int64_t full = s.g > 0 && s.g <= 64 ? 1024 : 512;
+  const int64_t full = s.g <= 64 ? tune("LN_W", 512) : s.g == 0 ? 512 : 256 * (s.g >= 512 ? 1 : tune("LN_B", 512) / s.g);
   return (int)(need < full ? need : full);
 }
 

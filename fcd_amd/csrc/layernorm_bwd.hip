@@ -5,41 +5,49 @@ namespace {
 
 // A row's x and gy in registers, one exchange for both of its sums, dx out; a thread meets the same columns in every row, so
 // the affine sums stay in its registers until the last row.  The next row's loads are in flight meanwhile.
-template <typename T, int G, int NV, bool EPI>
+// EPI 0: plain; 1: dropout; 2: activation, and dropout if there is any.
+template <typename T, int G, int NV, int EPI>
 __global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd_rows(LnArgs p) {
   constexpr int TH = G > 64 ? G : 256, RPB = TH / G, WAVES = RowSums<G, 2>::WAVES;
   __shared__ float sm[2 * 2 * WAVES];
   __shared__ float aff[affine_lds<G, NV>()];
   int turn = 0;
   if (EPI) drop_state(p.drop);
-  const int lane = threadIdx.x % G;
-  const float inv = 1.f / (float)p.cols;
+  const int lane = threadIdx.x % G, cols = (int)p.cols;
+  const float inv = 1.f / (float)cols;
   float ga[NV][8], be[NV][8], dg[NV][8], db[NV][8];
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    const long c = (lane + k * G) * 8;
-    load_param<T>(p.gamma, p.param_f32, c, p.cols - c, 1.f, ga[k]);
-    if (EPI) load_param<T>(p.beta, p.param_f32, c, p.cols - c, 0.f, be[k]);
+    const int c = (lane + k * G) * 8;
+    load_param<T>(p.gamma, p.param_f32, c, cols - c, 1.f, ga[k]);
+    if (EPI == 2) load_param<T>(p.beta, p.param_f32, c, cols - c, 0.f, be[k]);
 #pragma unroll
     for (int j = 0; j < 8; ++j) dg[k][j] = db[k][j] = 0.f;
   }
   typename Oct<T>::type nx[NV], ng[NV];
   float nmean = 0.f, nrstd = 0.f;
-  long row = (long)blockIdx.x * RPB + threadIdx.x / G;
   auto fetch = [&](long r) {
-    const bool here = r < p.rows;
+    const bool here = G >= 64 || r < p.rows;
     nmean = here ? p.mean[r] : 0.f;
     nrstd = here ? p.rstd[r] : 0.f;
+    const T *x = (const T*)p.x + r * p.ld_x, *gy = (const T*)p.gy + r * p.ld_gy;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const long c = (lane + k * G) * 8, n = here ? p.cols - c : 0;
-      load_raw<T>((const T*)p.x + r * p.ld_x + c, n, nx[k]);
-      load_raw<T>((const T*)p.gy + r * p.ld_gy + c, n, ng[k]);
+      const int c = (lane + k * G) * 8, n = here ? cols - c : 0;
+      if (n >= 8) {
+        nx[k] = *(const typename Oct<T>::type*)(x + c);
+        ng[k] = *(const typename Oct<T>::type*)(gy + c);
+      } else {
+        load_raw<T>(x + c, n, nx[k]);
+        load_raw<T>(gy + c, n, ng[k]);
+      }
     }
   };
-  fetch(row);
-  // every thread makes the same number of turns: the sums need whole groups
-  const long step = (long)gridDim.x * RPB, turns = (p.rows - (long)blockIdx.x * RPB + step - 1) / step;
+  // G < 64: every thread of a wave makes the same number of turns, for the sums need whole groups; G >= 64: whole waves do
+  long row = first_row<G, TH>();
+  const long step = (long)gridDim.x * RPB;
+  const long turns = (p.rows - (G >= 64 ? row : (long)blockIdx.x * RPB) + step - 1) / step;
+  if (turns > 0) fetch(row);
   for (long it = 0; it < turns; ++it, row += step) {
     const float mean = nmean, rstd = nrstd;
     float xh[NV][8], a[NV][8];
@@ -52,13 +60,25 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd_rows(LnArgs p) {
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      if (EPI && p.drop.t) drop_apply(p.drop, drop_keep8(p.drop, (uint64_t)(row * p.cols + (lane + k * G) * 8)), a[k]);
+      if (EPI && p.drop.t) {
+        uint32_t w[4];
+        drop_draw8(p.drop, (uint64_t)(row * cols + (lane + k * G) * 8), w);
+        drop_apply(p.drop, w, a[k]);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) xh[k][j] = (xh[k][j] - mean) * rstd;      // (absent elements: gy is 0, and so is what follows)
+      if (EPI == 2) {
+        float u[8], d1[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[j] = fmaf(xh[k][j], ga[k][j], be[k][j]);
+        ln_act8(u, p.act, nullptr, d1, nullptr);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) a[k][j] *= d1[j];
+      }
       float s0 = 0.f, s1 = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        xh[k][j] = (xh[k][j] - mean) * rstd;          // (absent elements: gy is 0, and so is all that follows)
-        float g1 = a[k][j];
-        if (EPI) g1 *= ln_act<1>(fmaf(xh[k][j], ga[k][j], be[k][j]), p.act);
+        const float g1 = a[k][j];
         dg[k][j] = fmaf(g1, xh[k][j], dg[k][j]);
         db[k][j] += g1;
         a[k][j] = g1 * ga[k][j];
@@ -69,13 +89,14 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd_rows(LnArgs p) {
       s[1] += s1;
     }
     RowSums<G, 2>::run(s, sm, turn);
-    const float am = s[0] * inv, ax = s[1] * inv;
+    const float c0 = -rstd * (s[0] * inv), c1 = -rstd * (s[1] * inv);
+    T* out = (T*)p.out + row * p.ld_out;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const long c = (lane + k * G) * 8, n = row < p.rows ? p.cols - c : 0;
+      const int c = (lane + k * G) * 8, n = G >= 64 || row < p.rows ? cols - c : 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) a[k][j] = rstd * (a[k][j] - am - xh[k][j] * ax);
-      store8((T*)p.out + row * p.ld_out + c, n, a[k]);
+      for (int j = 0; j < 8; ++j) a[k][j] = fmaf(a[k][j], rstd, fmaf(xh[k][j], c1, c0));
+      store8(out + c, n, a[k]);
     }
   }
   if (p.partial) write_partial<G, NV>(p, dg, db, aff);
@@ -94,7 +115,7 @@ __global__ __launch_bounds__(1024) void ln_bwd_long(LnArgs p) {
     float s[2] = {0.f, 0.f};
     for (long c = threadIdx.x * 8; c < p.cols; c += TH * 8) {
       Eight e;
-      load_eight<T>(p, row, c, mean, rstd, e);
+      load_eight<T, false>(p, row, c, mean, rstd, e);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         s[0] += e.a[j];
@@ -106,7 +127,7 @@ __global__ __launch_bounds__(1024) void ln_bwd_long(LnArgs p) {
     for (long c = threadIdx.x * 8; c < p.cols; c += TH * 8) {
       const long n = p.cols - c;
       Eight e;
-      load_eight<T>(p, row, c, mean, rstd, e);
+      load_eight<T, false>(p, row, c, mean, rstd, e);
       float dx[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) dx[j] = rstd * (e.a[j] - am - e.xh[j] * ax);
@@ -125,18 +146,18 @@ __global__ __launch_bounds__(1024) void ln_bwd_long(LnArgs p) {
 
 template <typename T>
 void launch(const LnArgs& a, int groups, hipStream_t st) {
-  const LnShape s = ln_shape(a.cols);
-  const bool epi = a.act != 1.f || a.drop.t;
+  const LnShape s = ln_bwd_shape(a.cols);
   if (s.g == 0) {
     ln_bwd_long<T><<<groups, 1024, 0, st>>>(a);
     return;
   }
-#define SHAPE(G, NV)                                                                            \
-  if (s.g == G && s.nv == NV) {                                                                 \
-    if (epi) ln_bwd_rows<T, G, NV, true><<<groups, G > 64 ? G : 256, 0, st>>>(a);               \
-    else ln_bwd_rows<T, G, NV, false><<<groups, G > 64 ? G : 256, 0, st>>>(a);                  \
+#define SHAPE(G, NV)                                                                                      \
+  if (s.g == G && s.nv == NV) {                                                                           \
+    if (a.act != 1.f) ln_bwd_rows<T, G, NV, 2><<<groups, G > 64 ? G : 256, 0, st>>>(a);                     \
+    else if (a.drop.t) ln_bwd_rows<T, G, NV, 1><<<groups, G > 64 ? G : 256, 0, st>>>(a);                    \
+    else ln_bwd_rows<T, G, NV, 0><<<groups, G > 64 ? G : 256, 0, st>>>(a);                                  \
   }
-  LN_FOR_EACH_SHAPE(SHAPE)
+  LN_BWD_SHAPES(SHAPE)
 #undef SHAPE
 }
 

@@ -3,63 +3,89 @@
 
 namespace {
 
-// A row's x, gy and v = ggx in registers; five sums in one exchange, two more if the activation is curved.
-template <typename T, int G, int NV, bool EPI>
+// A row's x, gy and v = ggx in registers; five sums in one exchange, two more if the activation is curved.  With the row's
+// sums in hand gx is a combination of four things: c0 + c1 t + c2 a + c3 xhat (+ rstd q gamma).
+// EPI 0: plain; 1: dropout; 2: activation, and dropout if there is any.
+template <typename T, int G, int NV, int EPI>
 __global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd2_rows(LnArgs p) {
   constexpr int TH = G > 64 ? G : 256, RPB = TH / G, WAVES = RowSums<G, 5>::WAVES;
   __shared__ float sm[2 * 5 * WAVES], sm2[2 * 2 * WAVES];
   __shared__ float aff[affine_lds<G, NV>()];
   int turn = 0, turn2 = 0;
   if (EPI) drop_state(p.drop);
-  const int lane = threadIdx.x % G;
-  const float inv = 1.f / (float)p.cols;
-  const bool smooth = EPI && p.act > 1.f;
+  const int lane = threadIdx.x % G, cols = (int)p.cols;
+  const float inv = 1.f / (float)cols;
+  const bool curved = EPI == 2 && p.act > 1.f;
   float ga[NV][8], be[NV][8], dg[NV][8], db[NV][8];
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    const long c = (lane + k * G) * 8;
-    load_param<T>(p.gamma, p.param_f32, c, p.cols - c, 1.f, ga[k]);
-    if (EPI) load_param<T>(p.beta, p.param_f32, c, p.cols - c, 0.f, be[k]);
+    const int c = (lane + k * G) * 8;
+    load_param<T>(p.gamma, p.param_f32, c, cols - c, 1.f, ga[k]);
+    if (EPI == 2) load_param<T>(p.beta, p.param_f32, c, cols - c, 0.f, be[k]);
 #pragma unroll
     for (int j = 0; j < 8; ++j) dg[k][j] = db[k][j] = 0.f;
   }
-  // every thread makes the same number of turns: the sums need whole groups
-  const long step = (long)gridDim.x * RPB, turns = (p.rows - (long)blockIdx.x * RPB + step - 1) / step;
-  long row = (long)blockIdx.x * RPB + threadIdx.x / G;
-  for (long it = 0; it < turns; ++it, row += step) {
-    const bool here = row < p.rows;
-    const float mean = here ? p.mean[row] : 0.f, rstd = here ? p.rstd[row] : 0.f;
-    typename Oct<T>::type rx[NV], rg[NV], rv[NV];
+  typename Oct<T>::type nx[NV], ng[NV], nv[NV];
+  float nmean = 0.f, nrstd = 0.f;
+  auto fetch = [&](long r) {
+    const bool here = G >= 64 || r < p.rows;
+    nmean = here ? p.mean[r] : 0.f;
+    nrstd = here ? p.rstd[r] : 0.f;
+    const T *x = (const T*)p.x + r * p.ld_x, *gy = (const T*)p.gy + r * p.ld_gy, *v = (const T*)p.ggx + r * p.ld_ggx;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const long c = (lane + k * G) * 8, n = here ? p.cols - c : 0;
-      load_raw<T>((const T*)p.x + row * p.ld_x + c, n, rx[k]);
-      load_raw<T>((const T*)p.gy + row * p.ld_gy + c, n, rg[k]);
-      load_raw<T>((const T*)p.ggx + row * p.ld_ggx + c, n, rv[k]);
+      const int c = (lane + k * G) * 8, n = here ? cols - c : 0;
+      if (n >= 8) {
+        nx[k] = *(const typename Oct<T>::type*)(x + c);
+        ng[k] = *(const typename Oct<T>::type*)(gy + c);
+        nv[k] = *(const typename Oct<T>::type*)(v + c);
+      } else {
+        load_raw<T>(x + c, n, nx[k]);
+        load_raw<T>(gy + c, n, ng[k]);
+        load_raw<T>(v + c, n, nv[k]);
+      }
     }
-    // xhat, drop(gy), v, and with an epilogue act'(u) and act''(u)
+  };
+  // G < 64: every thread of a wave makes the same number of turns, for the sums need whole groups; G >= 64: whole waves do
+  long row = first_row<G, TH>();
+  const long step = (long)gridDim.x * RPB;
+  const long turns = (p.rows - (G >= 64 ? row : (long)blockIdx.x * RPB) + step - 1) / step;
+  if (turns > 0) fetch(row);
+  for (long it = 0; it < turns; ++it, row += step) {
+    const float mean = nmean, rstd = nrstd;
+    // xhat, drop(gy), v, and behind an activation act'(u) and act''(u)
     float xh[NV][8], g[NV][8], v[NV][8], d1[NV][8], q[NV][8], s[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
-    uint32_t keep[NV];
+    uint32_t w[NV][4];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      widen<T>(rx[k], xh[k]);
-      widen<T>(rg[k], g[k]);
-      widen<T>(rv[k], v[k]);
-      keep[k] = 0xff;
+      widen<T>(nx[k], xh[k]);
+      widen<T>(ng[k], g[k]);
+      widen<T>(nv[k], v[k]);
+    }
+    if (it + 1 < turns) fetch(row + step);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
       if (EPI && p.drop.t) {
-        keep[k] = drop_keep8(p.drop, (uint64_t)(row * p.cols + (lane + k * G) * 8));
-        drop_apply(p.drop, keep[k], g[k]);
+        drop_draw8(p.drop, (uint64_t)(row * cols + (lane + k * G) * 8), w[k]);
+        drop_apply(p.drop, w[k], g[k]);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) xh[k][j] = (xh[k][j] - mean) * rstd;      // (absent elements: gy and v are 0)
+      if (EPI == 2) {
+        float u[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[j] = fmaf(xh[k][j], ga[k][j], be[k][j]);
+        ln_act8(u, p.act, nullptr, d1[k], q[k]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          q[k][j] *= g[k][j] * ga[k][j];
+          g[k][j] *= d1[k][j];                        // g1
+        }
       }
       float t[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        xh[k][j] = (xh[k][j] - mean) * rstd;          // (absent elements: gy and v are 0, and so are their products)
-        if (EPI) {
-          const float u = fmaf(xh[k][j], ga[k][j], be[k][j]);
-          d1[k][j] = ln_act<1>(u, p.act);
-          q[k][j] = smooth ? ln_act<2>(u, p.act) : 0.f;
-        }
-        const float a = (EPI ? g[k][j] * d1[k][j] : g[k][j]) * ga[k][j];
+        const float a = g[k][j] * ga[k][j];
         t[0] += a;
         t[1] = fmaf(a, xh[k][j], t[1]);
         t[2] += v[k][j];
@@ -72,14 +98,19 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd2_rows(LnArgs p) {
     RowSums<G, 5>::run(s, sm, turn);
     const float am = s[0] * inv, ax = s[1] * inv, vm = s[2] * inv, vx = s[3] * inv;
     const float sv = s[4] * inv - vm * am - vx * ax;
+    // t, the cotangent of a, in the place of v
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[k][j] = rstd * (v[k][j] - vm - xh[k][j] * vx);
     float q2[2] = {0.f, 0.f};
-    if (smooth) {
+    if (EPI == 2 && curved) {
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         float q0 = 0.f, q1 = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          q[k][j] *= g[k][j] * ga[k][j] * (rstd * (v[k][j] - vm - xh[k][j] * vx));
+          q[k][j] *= v[k][j];
           const float qg = q[k][j] * ga[k][j];
           q0 += qg;
           q1 = fmaf(qg, xh[k][j], q1);
@@ -89,26 +120,36 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd2_rows(LnArgs p) {
       }
       RowSums<G, 2>::run(q2, sm2, turn2);
     }
-    const float hm = q2[0] * inv - rstd * (vm * ax + am * vx), hx = q2[1] * inv - 2.f * rstd * vx * ax;
-    const float srr = sv * rstd * rstd;
+    // with v = t / rstd + mean(v) + xhat mean(v xhat) put into h:
+    const float c0 = rstd * (rstd * am * vx - q2[0] * inv), c1 = -rstd * ax, c2 = -rstd * rstd * vx;
+    const float c3 = -rstd * (q2[1] * inv + rstd * (sv - vx * ax));
+    T *ggy = (T*)p.ggy + row * p.ld_ggy, *out = (T*)p.out + row * p.ld_out;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const long c = (lane + k * G) * 8, n = here ? p.cols - c : 0;
+      const int c = (lane + k * G) * 8, n = G >= 64 || row < p.rows ? cols - c : 0;
       float gg[8], gx[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float t = rstd * (v[k][j] - vm - xh[k][j] * vx);
-        const float g1 = EPI ? g[k][j] * d1[k][j] : g[k][j];
-        const float qj = EPI ? q[k][j] : 0.f;
-        gg[j] = (EPI ? d1[k][j] * ga[k][j] : ga[k][j]) * t;
-        const float h = qj * ga[k][j] - rstd * (v[k][j] * ax + g1 * ga[k][j] * vx);
-        gx[j] = rstd * (h - hm - xh[k][j] * hx) - srr * xh[k][j];
-        dg[k][j] += g1 * t + qj * xh[k][j];           // (absent elements: g1 and q are 0)
-        db[k][j] += qj;
+        gg[j] = (EPI == 2 ? d1[k][j] * ga[k][j] : ga[k][j]) * v[k][j];
+        gx[j] = fmaf(v[k][j], c1, fmaf(g[k][j] * ga[k][j], c2, fmaf(xh[k][j], c3, c0)));
+        dg[k][j] = fmaf(g[k][j], v[k][j], dg[k][j]);  // (absent elements: g1 and q are 0)
+        if (EPI == 2) {
+          gx[j] = fmaf(q[k][j] * ga[k][j], rstd, gx[j]);
+          dg[k][j] = fmaf(q[k][j], xh[k][j], dg[k][j]);
+          db[k][j] += q[k][j];
+        }
       }
-      if (EPI && p.drop.t) drop_apply(p.drop, keep[k], gg);
-      store8((T*)p.ggy + row * p.ld_ggy + c, n, gg);
-      store8((T*)p.out + row * p.ld_out + c, n, gx);
+      if (EPI && p.drop.t) drop_apply(p.drop, w[k], gg);
+      if (n >= 8) {
+        typename Oct<T>::type o, r;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] = (T)gg[j], r[j] = (T)gx[j];
+        *(typename Oct<T>::type*)(ggy + c) = o;
+        *(typename Oct<T>::type*)(out + c) = r;
+      } else {
+        store8(ggy + c, n, gg);
+        store8(out + c, n, gx);
+      }
     }
   }
   if (p.partial) write_partial<G, NV>(p, dg, db, aff);
@@ -130,7 +171,7 @@ __global__ __launch_bounds__(1024) void ln_bwd2_long(LnArgs p) {
     for (long c = threadIdx.x * 8; c < p.cols; c += TH * 8) {
       Eight e;
       float v[8];
-      load_eight<T>(p, row, c, mean, rstd, e);
+      load_eight<T, true>(p, row, c, mean, rstd, e);
       load8((const T*)p.ggx + row * p.ld_ggx + c, p.cols - c, v);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -149,12 +190,12 @@ __global__ __launch_bounds__(1024) void ln_bwd2_long(LnArgs p) {
       for (long c = threadIdx.x * 8; c < p.cols; c += TH * 8) {
         Eight e;
         float v[8];
-        load_eight<T>(p, row, c, mean, rstd, e);
+        load_eight<T, true>(p, row, c, mean, rstd, e);
         load8((const T*)p.ggx + row * p.ld_ggx + c, p.cols - c, v);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float t = rstd * (v[j] - vm - e.xh[j] * vx);
-          const float qg = j < p.cols - c ? e.gy[j] * ln_act<2>(e.u[j], p.act) * e.ga[j] * t * e.ga[j] : 0.f;
+          const float qg = j < p.cols - c ? e.gy[j] * e.d2[j] * e.ga[j] * t * e.ga[j] : 0.f;
           q2[0] += qg;
           q2[1] += qg * e.xh[j];
         }
@@ -166,18 +207,18 @@ __global__ __launch_bounds__(1024) void ln_bwd2_long(LnArgs p) {
       const long n = p.cols - c;
       Eight e;
       float v[8], gg[8], gx[8], dg[8], q[8];
-      load_eight<T>(p, row, c, mean, rstd, e);
+      load_eight<T, true>(p, row, c, mean, rstd, e);
       load8((const T*)p.ggx + row * p.ld_ggx + c, n, v);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float t = rstd * (v[j] - vm - e.xh[j] * vx);
-        q[j] = smooth ? e.gy[j] * ln_act<2>(e.u[j], p.act) * e.ga[j] * t : 0.f;
-        gg[j] = ln_act<1>(e.u[j], p.act) * e.ga[j] * t;
+        q[j] = smooth ? e.gy[j] * e.d2[j] * e.ga[j] * t : 0.f;
+        gg[j] = e.d1[j] * e.ga[j] * t;
         const float h = q[j] * e.ga[j] - rstd * (v[j] * ax + e.a[j] * vx);
         gx[j] = rstd * (h - hm - e.xh[j] * hx) - sv * rstd * rstd * e.xh[j];
         dg[j] = e.g1[j] * t + q[j] * e.xh[j];
       }
-      if (p.drop.t) drop_apply(p.drop, e.keep, gg);
+      if (p.drop.t) drop_apply(p.drop, e.w, gg);
       if (p.partial) {
         float* part = p.partial + (long)blockIdx.x * 2 * p.cols + c;
         add_partial(part, n, row == blockIdx.x, dg);
@@ -191,18 +232,18 @@ __global__ __launch_bounds__(1024) void ln_bwd2_long(LnArgs p) {
 
 template <typename T>
 void launch(const LnArgs& a, int groups, hipStream_t st) {
-  const LnShape s = ln_shape(a.cols);
-  const bool epi = a.act != 1.f || a.drop.t;
+  const LnShape s = ln_bwd_shape(a.cols);
   if (s.g == 0) {
     ln_bwd2_long<T><<<groups, 1024, 0, st>>>(a);
     return;
   }
-#define SHAPE(G, NV)                                                                            \
-  if (s.g == G && s.nv == NV) {                                                                 \
-    if (epi) ln_bwd2_rows<T, G, NV, true><<<groups, G > 64 ? G : 256, 0, st>>>(a);              \
-    else ln_bwd2_rows<T, G, NV, false><<<groups, G > 64 ? G : 256, 0, st>>>(a);                 \
+#define SHAPE(G, NV)                                                                                      \
+  if (s.g == G && s.nv == NV) {                                                                           \
+    if (a.act != 1.f) ln_bwd2_rows<T, G, NV, 2><<<groups, G > 64 ? G : 256, 0, st>>>(a);                     \
+    else if (a.drop.t) ln_bwd2_rows<T, G, NV, 1><<<groups, G > 64 ? G : 256, 0, st>>>(a);                    \
+    else ln_bwd2_rows<T, G, NV, 0><<<groups, G > 64 ? G : 256, 0, st>>>(a);                                  \
   }
-  LN_FOR_EACH_SHAPE(SHAPE)
+  LN_BWD_SHAPES(SHAPE)
 #undef SHAPE
 }
 

@@ -12,44 +12,37 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_fwd_rows(LnArgs p) {
   __shared__ float sm[2 * WAVES];
   int turn = 0;
   if (EPI) drop_state(p.drop);
-  const int lane = threadIdx.x % G;
-  const float fcols = (float)p.cols;
+  const int lane = threadIdx.x % G, cols = (int)p.cols;
+  const float fcols = (float)cols;
   float ga[NV][8], be[NV][8];
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    const long c = (lane + k * G) * 8;
-    load_param<T>(p.gamma, p.param_f32, c, p.cols - c, 1.f, ga[k]);
-    load_param<T>(p.beta, p.param_f32, c, p.cols - c, 0.f, be[k]);
+    const int c = (lane + k * G) * 8;
+    load_param<T>(p.gamma, p.param_f32, c, cols - c, 1.f, ga[k]);
+    load_param<T>(p.beta, p.param_f32, c, cols - c, 0.f, be[k]);
   }
   typename Oct<T>::type nx[NV];
-  long row = (long)blockIdx.x * RPB + threadIdx.x / G;
+  auto fetch = [&](const void* t, long ld, long r, typename Oct<T>::type (&o)[NV]) {
+    const T* x = (const T*)t + r * ld;
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const long c = (lane + k * G) * 8;
-    load_raw<T>((const T*)p.x + row * p.ld_x + c, row < p.rows ? p.cols - c : 0, nx[k]);
-  }
-  // every thread makes the same number of turns: the sums need whole groups
-  const long step = (long)gridDim.x * RPB, turns = (p.rows - (long)blockIdx.x * RPB + step - 1) / step;
+    for (int k = 0; k < NV; ++k) {
+      const int c = (lane + k * G) * 8;
+      load_raw<T>(x + c, G >= 64 || r < p.rows ? cols - c : 0, o[k]);
+    }
+  };
+  // G < 64: every thread of a wave makes the same number of turns, for the sums need whole groups; G >= 64: whole waves do
+  long row = first_row<G, TH>();
+  const long step = (long)gridDim.x * RPB;
+  const long turns = (p.rows - (G >= 64 ? row : (long)blockIdx.x * RPB) + step - 1) / step;
+  if (turns > 0) fetch(p.x, p.ld_x, row, nx);
   for (long it = 0; it < turns; ++it, row += step) {
-    const bool here = row < p.rows;
+    const bool here = G >= 64 || row < p.rows;
     float v[NV][8];
 #pragma unroll
     for (int k = 0; k < NV; ++k) widen<T>(nx[k], v[k]);
     typename Oct<T>::type rs[NV];
-    if (EPI && p.res) {
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const long c = (lane + k * G) * 8;
-        load_raw<T>((const T*)p.res + row * p.ld_res + c, here ? p.cols - c : 0, rs[k]);
-      }
-    }
-    if (it + 1 < turns) {
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const long c = (lane + k * G) * 8;
-        load_raw<T>((const T*)p.x + (row + step) * p.ld_x + c, row + step < p.rows ? p.cols - c : 0, nx[k]);
-      }
-    }
+    if (EPI && p.res) fetch(p.res, p.ld_res, row, rs);
+    if (it + 1 < turns) fetch(p.x, p.ld_x, row + step, nx);
     float s[1] = {0.f};
 #pragma unroll
     for (int k = 0; k < NV; ++k)
@@ -59,7 +52,7 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_fwd_rows(LnArgs p) {
     s[0] = 0.f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const long n = p.cols - (lane + k * G) * 8;
+      const int n = cols - (lane + k * G) * 8;
       float q = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -74,25 +67,33 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_fwd_rows(LnArgs p) {
       p.mean[row] = mean;
       p.rstd[row] = rstd;
     }
+    T* out = (T*)p.out + row * p.ld_out;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const long c = (lane + k * G) * 8, n = here ? p.cols - c : 0;
+      const int c = (lane + k * G) * 8, n = here ? cols - c : 0;
+      float u[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[k][j] = fmaf(v[k][j] * rstd, ga[k][j], be[k][j]);
+      for (int j = 0; j < 8; ++j) u[j] = fmaf(v[k][j] * rstd, ga[k][j], be[k][j]);
       if (EPI) {
         if (p.act != 1.f) {
+          float a[8];
+          ln_act8(u, p.act, a, nullptr, nullptr);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[k][j] = ln_act<0>(v[k][j], p.act);
+          for (int j = 0; j < 8; ++j) u[j] = a[j];
         }
-        if (p.drop.t) drop_apply(p.drop, drop_keep8(p.drop, (uint64_t)(row * p.cols + c)), v[k]);
+        if (p.drop.t) {
+          uint32_t w[4];
+          drop_draw8(p.drop, (uint64_t)(row * cols + c), w);
+          drop_apply(p.drop, w, u);
+        }
         if (p.res) {
           float r[8];
           widen<T>(rs[k], r);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[k][j] += r[j];
+          for (int j = 0; j < 8; ++j) u[j] += r[j];
         }
       }
-      store8((T*)p.out + row * p.ld_out + c, n, v[k]);
+      store8(out + c, n, u);
     }
   }
 }
@@ -134,13 +135,18 @@ __global__ __launch_bounds__(1024) void ln_fwd_long(LnArgs p) {
     }
     for (long c = threadIdx.x * 8; c < p.cols; c += TH * 8) {
       const long n = p.cols - c;
-      float v[8], ga[8], be[8];
+      float v[8], u[8], ga[8], be[8];
       load8(x + c, n, v);
       load_param<T>(p.gamma, p.param_f32, c, n, 1.f, ga);
       load_param<T>(p.beta, p.param_f32, c, n, 0.f, be);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = ln_act<0>(fmaf((v[j] - mean) * rstd, ga[j], be[j]), p.act);
-      if (p.drop.t) drop_apply(p.drop, drop_keep8(p.drop, (uint64_t)(row * p.cols + c)), v);
+      for (int j = 0; j < 8; ++j) u[j] = fmaf((v[j] - mean) * rstd, ga[j], be[j]);
+      ln_act8(u, p.act, v, nullptr, nullptr);
+      if (p.drop.t) {
+        uint32_t w[4];
+        drop_draw8(p.drop, (uint64_t)(row * p.cols + c), w);
+        drop_apply(p.drop, w, v);
+      }
       if (p.res) {
         float r[8];
         load8((const T*)p.res + row * p.ld_res + c, n, r);
@@ -154,22 +160,20 @@ __global__ __launch_bounds__(1024) void ln_fwd_long(LnArgs p) {
 
 template <typename T>
 void launch(const LnArgs& a, hipStream_t st) {
-  const LnShape s = ln_shape(a.cols);
+  const int64_t units = (a.cols + 7) / 8;
   const bool epi = a.act != 1.f || a.drop.t || a.res;
-  if (s.g == 0) {
-    ln_fwd_long<T><<<(unsigned)(a.rows < 65536 ? a.rows : 65536), 1024, 0, st>>>(a);
-    return;
+#define SHAPE(G, NV)                                                        \
+  if (units <= G * NV) {                                                    \
+    const int th = G > 64 ? G : 256;                                        \
+    const long need = (a.rows + th / G - 1) / (th / G), full = 256 * (2048 / th); \
+    const unsigned grid = (unsigned)(need < full ? need : full);            \
+    if (epi) ln_fwd_rows<T, G, NV, true><<<grid, th, 0, st>>>(a);           \
+    else ln_fwd_rows<T, G, NV, false><<<grid, th, 0, st>>>(a);              \
+    return;                                                                 \
   }
-  const int th = s.g > 64 ? s.g : 256;
-  const long need = (a.rows + th / s.g - 1) / (th / s.g), full = 256 * (2048 / th);
-  const unsigned grid = (unsigned)(need < full ? need : full);
-#define SHAPE(G, NV)                                                  \
-  if (s.g == G && s.nv == NV) {                                       \
-    if (epi) ln_fwd_rows<T, G, NV, true><<<grid, th, 0, st>>>(a);     \
-    else ln_fwd_rows<T, G, NV, false><<<grid, th, 0, st>>>(a);        \
-  }
-  LN_FOR_EACH_SHAPE(SHAPE)
+  LN_FWD_SHAPES(SHAPE)
 #undef SHAPE
+  ln_fwd_long<T><<<(unsigned)(a.rows < 65536 ? a.rows : 65536), 1024, 0, st>>>(a);
 }
 
 }  // namespace
