@@ -17,11 +17,12 @@ struct LnArgs {
 int ln_check(const char* who, const FcdLayerNormDesc* d, LnArgs* a);
 int ln_check_vectors(const char* who, const FcdLayerNormDesc* d, const void* gamma, const void* beta, const void* mean,
                      const void* rstd);
-int ln_check_affine(const char* who, const FcdLayerNormDesc* d, const void* dgamma, const void* dbeta, void* workspace,
+int ln_check_affine(const char* who, const FcdLayerNormDesc* d, int second, const void* dgamma, const void* dbeta, void* workspace,
                     size_t workspace_bytes, LnArgs* a);
 int ln_finish(const char* who, const FcdLayerNormDesc* d, const LnArgs& a, int groups, void* dgamma, void* dbeta, int accumulate,
               hipStream_t st);
 int ln_groups(int64_t rows, int64_t cols);   // workgroups of the backward passes
+bool ln_few_rows(int64_t rows, int64_t cols);   // the first backward pass sums its columns beside the rows, in one launch
 
 // Where a row lives: G threads with NV units of 8 elements each.  G <= 64: the row's sums stay inside a wave, and a workgroup
 // of 256 works on 256 / G rows with no barrier; G > 64: one workgroup per row, one barrier per sum.  Longer rows than the last
@@ -88,6 +89,20 @@ __device__ __forceinline__ float dpp(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
 }
 
+// a + b after the exchange of a's upper half with b's lower half: sums of a's halves in the lower 32 lanes, of b's in the upper.
+__device__ __forceinline__ float swap32_add(float a, float b) {
+  const auto s = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), false, false);
+  const unsigned lo = s[0], hi = s[1];
+  return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+}
+
+// The same between odd rows of a and even rows of b (16 lanes each): rows 0 and 2 get sums of a's rows, 1 and 3 of b's.
+__device__ __forceinline__ float swap16_add(float a, float b) {
+  const auto s = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), false, false);
+  const unsigned lo = s[0], hi = s[1];
+  return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+}
+
 // Sum over groups of G neighbouring lanes, in every lane: swaps inside quads, mirrors of 8 and 16 lanes (all lanes of a
 // smaller group already hold the same value there), then the row and half swaps of gfx950.  No LDS round trip.
 template <int G>
@@ -96,38 +111,62 @@ __device__ __forceinline__ float lanes_sum(float v) {
   if constexpr (G >= 4) v += dpp<0x4E>(v);
   if constexpr (G >= 8) v += dpp<0x141>(v);
   if constexpr (G >= 16) v += dpp<0x140>(v);
-  if constexpr (G >= 32) {
-    const auto s = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
-    const unsigned lo = s[0], hi = s[1];
-    v = __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
-  }
-  if constexpr (G >= 64) {
-    const auto s = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
-    const unsigned lo = s[0], hi = s[1];
-    v = __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
-  }
+  if constexpr (G >= 32) v = swap16_add(v, v);
+  if constexpr (G >= 64) v = swap32_add(v, v);
   return v;
 }
 
-// Sums of K values over the G threads of a row, in every thread.  More than a wave: one barrier; `turn` alternates between two
-// buffers, and a wave writes to one again only behind the barrier of the other, which every wave reaches after its reads.
+__device__ __forceinline__ float lane_value(float v, int lane) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
+
+// Sums of K values over the G threads of a row, in every thread (from a wave on in scalar registers).  A wave's sums share
+// their exchanges: each swap folds two of them at once, so that five cost 21 instructions and not 50, and end up in the lanes
+// home(k).  More than a wave: one barrier; `turn` alternates between two buffers, and a wave writes to one again only behind
+// the barrier of the other, which every wave reaches after its reads.
 template <int G, int K>
 struct RowSums {
+  static_assert(K == 1 || K == 2 || K == 5, "");
   static constexpr int WAVES = G > 64 ? G / 64 : 1;
+  __device__ __forceinline__ static constexpr int home(int k) { return K == 1 ? 0 : K == 2 ? 32 * k : k < 4 ? 32 * (k & 1) + 8 * (k & 2) : 1; }
+
+  __device__ __forceinline__ static float fold(const float (&s)[K]) {
+    if constexpr (K == 1) return lanes_sum<64>(s[0]);
+    if constexpr (K == 2) {
+      const float r = swap32_add(s[0], s[1]);
+      return lanes_sum<16>(swap16_add(r, r));
+    }
+    if constexpr (K == 5) {
+      const float r = lanes_sum<16>(swap16_add(swap32_add(s[0], s[1]), swap32_add(s[2], s[3]))), t = lanes_sum<64>(s[4]);
+      return (threadIdx.x & 63) == 1 ? t : r;
+    }
+  }
+
   __device__ __forceinline__ static void run(float (&s)[K], float* sm, int& turn) {
+    if constexpr (G < 64) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) s[k] = lanes_sum<(G < 64 ? G : 64)>(s[k]);
-    if constexpr (G > 64) {
-      float* buf = sm + turn * WAVES * K;
-      turn ^= 1;
-      const int w = threadIdx.x >> 6;
-      if ((threadIdx.x & 63) == 0) {
+      for (int k = 0; k < K; ++k) s[k] = lanes_sum<G>(s[k]);
+    } else {
+      const float r = fold(s);
+      if constexpr (G == 64) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) buf[w * K + k] = s[k];
+        for (int k = 0; k < K; ++k) s[k] = lane_value(r, home(k));
+      } else {
+        float* buf = sm + turn * WAVES * K;
+        turn ^= 1;
+        const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+        int mine = -1;
+#pragma unroll
+        for (int k = 0; k < K; ++k) mine = lane == home(k) ? k : mine;
+        if (mine >= 0) buf[mine * WAVES + w] = r;
+        __syncthreads();
+        // sum k's waves in WAVES neighbouring lanes
+        constexpr int FIRST = K * WAVES < 64 ? K * WAVES : 64;
+        const float a = lanes_sum<WAVES>(buf[lane < FIRST ? lane : 0]);
+#pragma unroll
+        for (int k = 0; k < K && k * WAVES < 64; ++k) s[k] = lane_value(a, k * WAVES);
+        if constexpr (K * WAVES > 64) s[4] = lane_value(lanes_sum<WAVES>(buf[64 + (lane & (WAVES - 1))]), 0);
       }
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < K; ++k) s[k] = lanes_sum<WAVES>(buf[(threadIdx.x & (WAVES - 1)) * K + k]);
     }
   }
 };
@@ -140,15 +179,7 @@ __device__ __forceinline__ float fast_exp(float u) { return __builtin_amdgcn_exp
 
 // The activation (d0) of 8 values, or its first (d1) and second (d2) derivative; what is NULL is not computed.
 __device__ __forceinline__ void ln_act8(const float (&u)[8], float code, float* d0, float* d1, float* d2) {
-  if (code <= 1.f) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float s = u[j] > 0.f ? 1.f : code;
-      if (d0) d0[j] = u[j] * s;
-      if (d1) d1[j] = s;
-      if (d2) d2[j] = 0.f;
-    }
-  } else if (code == FCD_ACT_SILU) {
+  if (code == FCD_ACT_SILU) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float sg = __builtin_amdgcn_rcpf(1.f + fast_exp(-u[j])), ns = 1.f - sg;
@@ -156,7 +187,7 @@ __device__ __forceinline__ void ln_act8(const float (&u)[8], float code, float* 
       if (d1) d1[j] = fmaf(u[j] * sg, ns, sg);
       if (d2) d2[j] = sg * ns * fmaf(u[j], ns - sg, 2.f);
     }
-  } else {
+  } else if (code == FCD_ACT_MISH) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float e = fast_exp(fminf(u[j], 20.f)), n = e * (e + 2.f), r = __builtin_amdgcn_rcpf(n + 2.f), th = n * r;
@@ -167,6 +198,14 @@ __device__ __forceinline__ void ln_act8(const float (&u)[8], float code, float* 
         const float sg = e * __builtin_amdgcn_rcpf(1.f + e);
         d2[j] = w * fmaf(u[j], (1.f - sg) - 2.f * th * sg, 2.f);
       }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float s = u[j] > 0.f ? 1.f : code;
+      if (d0) d0[j] = u[j] * s;
+      if (d1) d1[j] = s;
+      if (d2) d2[j] = 0.f;
     }
   }
 }

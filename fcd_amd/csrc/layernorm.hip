@@ -44,8 +44,13 @@ static int64_t tune(const char* n, int64_t v) { const char* e = getenv(n); retur
 int ln_groups(int64_t rows, int64_t cols) {
   const LnShape s = ln_bwd_shape(cols);
   const int64_t rpb = s.g > 0 && s.g <= 64 ? 256 / s.g : 1, need = (rows + rpb - 1) / rpb;
-  const int64_t full = s.g <= 64 ? tune("LN_W", 512) : s.g == 0 ? 512 : 256 * (s.g >= 512 ? 1 : tune("LN_B", 512) / s.g);
+  const int64_t full = s.g <= 64 ? tune("LN_W", 512) : s.g == 0 ? 512 : 256 * (s.g >= tune("LN_B", 512) ? 1 : tune("LN_B", 512) / s.g);
   return (int)(need < full ? need : full);
+}
+
+bool ln_few_rows(int64_t rows, int64_t cols) {
+  const LnShape s = ln_bwd_shape(cols);
+  return s.g && rows > 0 && rows <= (s.g > 256 ? s.g : 256) / 2;   // four turns of a column workgroup
 }
 
 int ln_finish(const char* who, const FcdLayerNormDesc* d, const LnArgs& a, int groups, void* dgamma, void* dbeta, int accumulate,
@@ -55,15 +60,16 @@ int ln_finish(const char* who, const FcdLayerNormDesc* d, const LnArgs& a, int g
   return reduce<f16_t>(who, a, groups, dgamma, dbeta, accumulate, st);
 }
 
-int ln_check_affine(const char* who, const FcdLayerNormDesc* d, const void* dgamma, const void* dbeta, void* workspace,
+int ln_check_affine(const char* who, const FcdLayerNormDesc* d, int second, const void* dgamma, const void* dbeta, void* workspace,
                     size_t workspace_bytes, LnArgs* a) {
   FCD_TRY(ln_check_vectors(who, d, dgamma, dbeta, nullptr, nullptr));
   if (!dgamma && !dbeta) return FCD_OK;
-  if (workspace_bytes < fcd_layernorm_workspace_bytes(d)) {
-    fcd_set_error("%s: workspace of %zu bytes, needs %zu", who, workspace_bytes, fcd_layernorm_workspace_bytes(d));
+  const size_t need = fcd_layernorm_workspace_bytes(d, second);
+  if (workspace_bytes < need) {
+    fcd_set_error("%s: workspace of %zu bytes, needs %zu", who, workspace_bytes, need);
     return FCD_EWORKSPACE;
   }
-  FCD_REQUIRE(d->rows == 0 || (workspace && ((uintptr_t)workspace & 15u) == 0), "%s: workspace is NULL or not 16-byte aligned", who);
+  FCD_REQUIRE(need == 0 || (workspace && ((uintptr_t)workspace & 15u) == 0), "%s: workspace is NULL or not 16-byte aligned", who);
   a->partial = (float*)workspace;
   return FCD_OK;
 }
@@ -98,7 +104,7 @@ int ln_check_vectors(const char* who, const FcdLayerNormDesc* d, const void* gam
 
 extern "C" int fcd_layernorm_desc_bytes(void) { return (int)sizeof(FcdLayerNormDesc); }
 
-extern "C" size_t fcd_layernorm_workspace_bytes(const FcdLayerNormDesc* d) {
-  if (!d || d->rows <= 0 || d->cols <= 0) return 0;
+extern "C" size_t fcd_layernorm_workspace_bytes(const FcdLayerNormDesc* d, int second) {
+  if (!d || d->rows <= 0 || d->cols <= 0 || (!second && ln_few_rows(d->rows, d->cols))) return 0;
   return (size_t)ln_groups(d->rows, d->cols) * 2 * (size_t)d->cols * sizeof(float);
 }

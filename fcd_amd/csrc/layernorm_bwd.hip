@@ -6,11 +6,11 @@ namespace {
 // A row's x and gy in registers, one exchange for both of its sums, dx out; a thread meets the same columns in every row, so
 // the affine sums stay in its registers until the last row.  The next row's loads are in flight meanwhile.
 // EPI 0: plain; 1: dropout; 2: activation, and dropout if there is any.
-template <typename T, int G, int NV, int EPI>
-__global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd_rows(LnArgs p) {
+// (`blocks` workgroups from the first on; AFFINE: the affine sums are kept.)
+template <typename T, int G, int NV, int EPI, bool AFFINE>
+__device__ __forceinline__ void bwd_rows(LnArgs p, unsigned blocks) {
   constexpr int TH = G > 64 ? G : 256, RPB = TH / G, WAVES = RowSums<G, 2>::WAVES;
   __shared__ float sm[2 * 2 * WAVES];
-  __shared__ float aff[affine_lds<G, NV>()];
   int turn = 0;
   if (EPI) drop_state(p.drop);
   const int lane = threadIdx.x % G, cols = (int)p.cols;
@@ -45,7 +45,7 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd_rows(LnArgs p) {
   };
   // G < 64: every thread of a wave makes the same number of turns, for the sums need whole groups; G >= 64: whole waves do
   long row = first_row<G, TH>();
-  const long step = (long)gridDim.x * RPB;
+  const long step = (long)blocks * RPB;
   const long turns = (p.rows - (G >= 64 ? row : (long)blockIdx.x * RPB) + step - 1) / step;
   if (turns > 0) fetch(row);
   for (long it = 0; it < turns; ++it, row += step) {
@@ -79,8 +79,10 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd_rows(LnArgs p) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float g1 = a[k][j];
-        dg[k][j] = fmaf(g1, xh[k][j], dg[k][j]);
-        db[k][j] += g1;
+        if (AFFINE) {
+          dg[k][j] = fmaf(g1, xh[k][j], dg[k][j]);
+          db[k][j] += g1;
+        }
         a[k][j] = g1 * ga[k][j];
         s0 += a[k][j];
         s1 = fmaf(a[k][j], xh[k][j], s1);
@@ -99,7 +101,100 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd_rows(LnArgs p) {
       store8(out + c, n, a[k]);
     }
   }
-  if (p.partial) write_partial<G, NV>(p, dg, db, aff);
+  if constexpr (AFFINE) {
+    __shared__ float aff[affine_lds<G, NV>()];
+    if (p.partial) write_partial<G, NV>(p, dg, db, aff);
+  }
+}
+
+template <typename T, int G, int NV, int EPI>
+__global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd_rows(LnArgs p) {
+  bwd_rows<T, G, NV, EPI, true>(p, gridDim.x);
+}
+
+struct Affine {
+  void *dgamma, *dbeta;
+  int accumulate;
+};
+
+template <typename T>
+__device__ __forceinline__ void put_affine(void* out, int f32, int accumulate, int c, float v) {
+  if (!out) return;
+  if (f32) {
+    float* o = (float*)out + c;
+    *o = accumulate ? *o + v : v;
+  } else {
+    T* o = (T*)out + c;
+    *o = (T)(accumulate ? (float)*o + v : v);
+  }
+}
+
+// Few rows: the first `blocks` workgroups write dx; the others sum 64 columns each over all rows, which needs nothing from the
+// first ones (the row sums do not enter the affine gradients).  x and gy are read twice, from cache; in exchange there is
+// no scratch and no second launch.
+template <typename T, int G, int EPI>
+__global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd_few(LnArgs p, Affine f, unsigned blocks) {
+  constexpr int TH = G > 64 ? G : 256;
+  if (blockIdx.x < blocks) {
+    bwd_rows<T, G, 1, EPI, false>(p, blocks);
+    return;
+  }
+  __shared__ float sm[TH / 64][8][16];
+  if (EPI) drop_state(p.drop);
+  const int unit = threadIdx.x & 7, cols = (int)p.cols, c = ((int)(blockIdx.x - blocks) * 8 + unit) * 8, n = cols - c;
+  float ga[8], be[8], dg[8], db[8];
+  if (EPI == 2) {
+    load_param<T>(p.gamma, p.param_f32, c, n, 1.f, ga);
+    load_param<T>(p.beta, p.param_f32, c, n, 0.f, be);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) dg[j] = db[j] = 0.f;
+  for (long row = threadIdx.x >> 3; row < p.rows; row += TH / 8) {
+    const float mean = p.mean[row], rstd = p.rstd[row];
+    float xh[8], g[8];
+    load8((const T*)p.x + row * p.ld_x + c, n, xh);
+    load8((const T*)p.gy + row * p.ld_gy + c, n, g);
+    if (EPI && p.drop.t) {
+      uint32_t w[4];
+      drop_draw8(p.drop, (uint64_t)(row * cols + c), w);
+      drop_apply(p.drop, w, g);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) xh[j] = (xh[j] - mean) * rstd;
+    if (EPI == 2) {
+      float u[8], d1[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) u[j] = fmaf(xh[j], ga[j], be[j]);
+      ln_act8(u, p.act, nullptr, d1, nullptr);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[j] *= d1[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      dg[j] = fmaf(g[j], xh[j], dg[j]);
+      db[j] += g[j];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+#pragma unroll
+    for (int o = 8; o < 64; o <<= 1) {
+      dg[j] += __shfl_xor(dg[j], o, 64);
+      db[j] += __shfl_xor(db[j], o, 64);
+    }
+    if ((threadIdx.x & 63) < 8) {
+      sm[threadIdx.x >> 6][unit][j] = dg[j];
+      sm[threadIdx.x >> 6][unit][8 + j] = db[j];
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < 128) {
+    const int which = threadIdx.x >> 6, i = threadIdx.x & 63, col = (int)(blockIdx.x - blocks) * 64 + i;
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < TH / 64; ++w) s += sm[w][i >> 3][which * 8 + (i & 7)];
+    if (col < cols) put_affine<T>(which ? f.dbeta : f.dgamma, p.param_f32, f.accumulate, col, s);
+  }
 }
 
 // Rows too long for registers: both operands read again for every pass, the affine sums kept in the scratch.
@@ -161,6 +256,20 @@ void launch(const LnArgs& a, int groups, hipStream_t st) {
 #undef SHAPE
 }
 
+template <typename T>
+void launch_few(const LnArgs& a, const Affine& f, int groups, hipStream_t st) {
+  const LnShape s = ln_bwd_shape(a.cols);
+  const unsigned grid = groups + (unsigned)((a.cols + 63) / 64);
+#define SHAPE(G, NV)                                                                                      \
+  if (s.g == G) {                                                                                         \
+    if (a.act != 1.f) ln_bwd_few<T, G, 2><<<grid, G > 64 ? G : 256, 0, st>>>(a, f, groups);               \
+    else if (a.drop.t) ln_bwd_few<T, G, 1><<<grid, G > 64 ? G : 256, 0, st>>>(a, f, groups);              \
+    else ln_bwd_few<T, G, 0><<<grid, G > 64 ? G : 256, 0, st>>>(a, f, groups);                            \
+  }
+  LN_BWD_SHAPES(SHAPE)
+#undef SHAPE
+}
+
 }  // namespace
 
 extern "C" int fcd_layernorm_bwd(const FcdLayerNormDesc* d, const void* gy, const void* x, const float* mean, const float* rstd,
@@ -178,10 +287,17 @@ extern "C" int fcd_layernorm_bwd(const FcdLayerNormDesc* d, const void* gy, cons
   FCD_TRY(fcd_check_apart(who, vo, vg, d->rows, d->cols, es, true));
   FCD_TRY(ln_check_vectors(who, d, gamma, beta, mean, rstd));
   FCD_REQUIRE(d->rows == 0 || (mean && rstd), "%s: mean / rstd are NULL", who);
-  FCD_TRY(ln_check_affine(who, d, dgamma, dbeta, workspace, workspace_bytes, &a));
+  FCD_TRY(ln_check_affine(who, d, 0, dgamma, dbeta, workspace, workspace_bytes, &a));
   a.x = x, a.gy = gy, a.gamma = gamma, a.beta = beta, a.out = dx, a.mean = (float*)mean, a.rstd = (float*)rstd;
   const int groups = ln_groups(d->rows, d->cols);
   hipStream_t st = fcd_stream(stream);
+  if ((dgamma || dbeta) && ln_few_rows(d->rows, d->cols)) {
+    const Affine f{dgamma, dbeta, accumulate};
+    if (d->dtype == FCD_DT_F32) launch_few<float>(a, f, groups, st);
+    else if (d->dtype == FCD_DT_BF16) launch_few<bf16_t>(a, f, groups, st);
+    else launch_few<f16_t>(a, f, groups, st);
+    return fcd_check_launch(who);
+  }
   if (d->rows) {
     if (d->dtype == FCD_DT_F32) launch<float>(a, groups, st);
     else if (d->dtype == FCD_DT_BF16) launch<bf16_t>(a, groups, st);

@@ -266,7 +266,7 @@ extern "C" int fcd_layernorm_bwd2(const FcdLayerNormDesc* d, const void* ggx, co
   FCD_TRY(fcd_check_apart(who, out[0], out[1], d->rows, d->cols, es, false));
   FCD_TRY(ln_check_vectors(who, d, gamma, beta, mean, rstd));
   FCD_REQUIRE(d->rows == 0 || (mean && rstd), "%s: mean / rstd are NULL", who);
-  FCD_TRY(ln_check_affine(who, d, dgamma, dbeta, workspace, workspace_bytes, &a));
+  FCD_TRY(ln_check_affine(who, d, 1, dgamma, dbeta, workspace, workspace_bytes, &a));
   a.x = x, a.gy = gy, a.ggx = ggx, a.gamma = gamma, a.beta = beta, a.out = gx, a.ggy = ggy;
   a.mean = (float*)mean, a.rstd = (float*)rstd;
   const int groups = ln_groups(d->rows, d->cols);

@@ -770,23 +770,31 @@ def _rows(t: torch.Tensor, name: str):
 
 def _row_operand(t: torch.Tensor, name: str, like: torch.Tensor) -> int:
     """Row stride of ``t``, which goes with ``like`` (same shape, type and device)."""
-    if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
+    if t.shape != like.shape or t.dtype != like.dtype or t.get_device() != like.get_device():
         raise RuntimeError(f"fcd_amd: {name} is {t.dtype} {tuple(t.shape)} on {t.device}, "
                            f"expected {like.dtype} {tuple(like.shape)} on {like.device}")
     return _rows(t, name)[2]
 
 
-def _require_here(t: torch.Tensor, name: str) -> None:
-    if not t.is_cuda:
-        raise RuntimeError(f"fcd_amd: {name} must live on the GPU (got {t.device}); the HIP path has no CPU fallback")
-    if t.get_device() != torch._C._cuda_getDevice():
+def _here(t: torch.Tensor, name: str) -> int:
+    """FCD_DT_* of a tensor on the current device."""
+    dt, dev = _DT.get(t.dtype), t.get_device()
+    if dt is None or dev < 0 or dev != torch._C._cuda_getDevice():
+        if dev < 0:
+            raise RuntimeError(f"fcd_amd: {name} must live on the GPU (got {t.device}); the HIP path has no CPU fallback")
+        if dt is None:
+            raise RuntimeError(f"fcd_amd: {name} must be float32, bfloat16 or float16 (got {t.dtype})")
         raise RuntimeError(f"fcd_amd: {name} is on {t.device}, the current device is cuda:{torch._C._cuda_getDevice()}")
-    if t.dtype not in _DT:
-        raise RuntimeError(f"fcd_amd: {name} must be float32, bfloat16 or float16 (got {t.dtype})")
+    return dt
 
 
-def _rng_words(p: float, rng, device):
-    """(seed, offset, device address) for the C calls."""
+def _fresh(t: torch.Tensor) -> torch.Tensor:
+    """An uninitialised contiguous tensor like ``t``."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+def _rng_words(p: float, rng, device: int):
+    """(seed, offset, device address) for the C calls; ``device``: index of the operands' device."""
     if not 0.0 <= p <= 1.0:
         raise RuntimeError(f"fcd_amd: the dropout probability must be in [0, 1] (got {p})")
     if p == 0.0:
@@ -794,7 +802,7 @@ def _rng_words(p: float, rng, device):
     if rng is None:
         raise RuntimeError("fcd_amd: dropout needs rng: (seed, offset) or what dropout_take returned")
     if isinstance(rng, torch.Tensor):
-        if rng.dtype != torch.int64 or rng.numel() != 2 or not rng.is_contiguous() or rng.device != device:
+        if rng.dtype != torch.int64 or rng.numel() != 2 or not rng.is_contiguous() or rng.get_device() != device:
             raise RuntimeError("fcd_amd: a dropout rng tensor is two contiguous int64 words on the operands' device")
         return 0, 0, rng.data_ptr()
     seed, offset = rng
@@ -830,64 +838,69 @@ def dropout(x: torch.Tensor, p: float, rng, residual: Optional[torch.Tensor] = N
     stored: the backward pass is the same call on the gradient (without ``residual``).  ``rng`` is ``(seed, offset)`` or
     what :func:`dropout_take` returned; ``numel`` elements use ``ceil(numel / 8)`` offsets.  ``p`` is resolved to 2^-16.
     float32, bfloat16, float16; rows may be strided; ``out`` may be ``x``."""
-    _require_here(x, "x")
+    dt = _here(x, "x")
     rows, cols, ld = _rows(x, "x")
-    seed, offset, words = _rng_words(p, rng, x.device)
+    seed, offset, words = _rng_words(p, rng, x.get_device())
     ld_r = 0 if residual is None else _row_operand(residual, "residual", x)
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        ld_o = cols
+        out, ld_o = _fresh(x), cols
     else:
         ld_o = _row_operand(out, "out", x)
-    check(L.load().fcd_dropout(x.data_ptr(), ptr(residual), out.data_ptr(), rows, cols, ld, ld_r, ld_o, _DT[x.dtype], p, seed,
-                               offset, words, stream()), "dropout")
+    check(L.load().fcd_dropout(x.data_ptr(), ptr(residual), out.data_ptr(), rows, cols, ld, ld_r, ld_o, dt, p, seed, offset,
+                               words, stream()), "dropout")
     return out
 
 
+def _ln_param(t, name, cols, x):
+    if (t.dtype != torch.float32 and t.dtype != x.dtype) or t.get_device() != x.get_device() or t.numel() != cols \
+            or not t.is_contiguous():
+        raise RuntimeError(f"fcd_amd: {name} must be a contiguous float32 or {x.dtype} vector of {cols} elements on {x.device}")
+    return _DT[t.dtype]
+
+
 def _ln_desc(x, gamma, beta, eps, act_slope, p, rng):
-    _require_here(x, "x")
     d = L.LayerNormDesc()
-    d.rows, d.cols, d.ld_x = _rows(x, "x")
-    d.dtype = d.param_dtype = _DT[x.dtype]
-    if gamma is None and beta is None:
-        d.param_dtype = 0
-    for t, name in ((gamma, "gamma"), (beta, "beta")):
-        if t is not None:
-            if t.dtype not in (torch.float32, x.dtype) or t.device != x.device or t.numel() != d.cols or not t.is_contiguous():
-                raise RuntimeError(f"fcd_amd: {name} must be a contiguous float32 or {x.dtype} vector of {d.cols} elements "
-                                   f"on {x.device}")
-            d.param_dtype = _DT[t.dtype]
-    if gamma is not None and beta is not None and gamma.dtype != beta.dtype:
-        raise RuntimeError("fcd_amd: gamma and beta must have one type")
+    d.dtype = _here(x, "x")
+    d.rows, cols, d.ld_x = _rows(x, "x")
+    d.cols = cols
+    if gamma is not None:
+        d.param_dtype = _ln_param(gamma, "gamma", cols, x)
+    if beta is not None:
+        dt = _ln_param(beta, "beta", cols, x)
+        if gamma is not None and dt != d.param_dtype:
+            raise RuntimeError("fcd_amd: gamma and beta must have one type")
+        d.param_dtype = dt
     d.eps, d.act, d.drop_p = eps, act_slope, p
-    d.seed, d.offset, d.rng = _rng_words(p, rng, x.device)
+    if p != 0.0:
+        d.seed, d.offset, d.rng = _rng_words(p, rng, x.get_device())
     return d
 
 
 def _ln_stat(t, name, d, x):
-    if t.dtype != torch.float32 or t.device != x.device or t.numel() != d.rows or not t.is_contiguous():
+    if t.dtype != torch.float32 or t.get_device() != x.get_device() or t.numel() != d.rows or not t.is_contiguous():
         raise RuntimeError(f"fcd_amd: {name} must be a contiguous float32 vector of {d.rows} elements on {x.device}")
     return t.data_ptr()
 
 
-def _ln_affine(gamma, beta, want_affine, dgamma, dbeta, accumulate, d, x):
+def _ln_affine(gamma, beta, want_affine, dgamma, dbeta, accumulate, d, x, second):
     """Gradient tensors of the affine parameters (given, fresh, or None) and the scratch their row sums need."""
-    if want_affine and dgamma is None and dbeta is None:
+    if not want_affine:
+        return None, None, None, 0
+    if dgamma is None and dbeta is None:
         if accumulate:
             raise RuntimeError("fcd_amd: accumulate needs dgamma / dbeta")
         dgamma = None if gamma is None else torch.empty_like(gamma)
         dbeta = None if beta is None else torch.empty_like(beta)
-    elif not want_affine:
-        dgamma = dbeta = None
-    for t, name in ((dgamma, "dgamma"), (dbeta, "dbeta")):
-        if t is not None and (_DT.get(t.dtype) != d.param_dtype or t.device != x.device or t.numel() != d.cols
-                              or not t.is_contiguous()):
-            raise RuntimeError(f"fcd_amd: {name} must be a contiguous vector of {d.cols} elements of the parameters' type")
-    ws = None
-    if dgamma is not None or dbeta is not None:
-        # a buffer of this call's own: inside a captured graph it belongs to that graph's memory
-        ws = torch.empty(L.load().fcd_layernorm_workspace_bytes(C.byref(d)), dtype=torch.uint8, device=x.device)
-    return dgamma, dbeta, ws, 0 if ws is None else ws.numel()
+    else:
+        for t, name in ((dgamma, "dgamma"), (dbeta, "dbeta")):
+            if t is not None and (_DT.get(t.dtype) != d.param_dtype or t.get_device() != x.get_device()
+                                  or t.numel() != d.cols or not t.is_contiguous()):
+                raise RuntimeError(f"fcd_amd: {name} must be a contiguous vector of {d.cols} elements of the parameters' type")
+    if dgamma is None and dbeta is None:
+        return None, None, None, 0
+    n = L.load().fcd_layernorm_workspace_bytes(C.byref(d), second)
+    # a buffer of this call's own: inside a captured graph it belongs to that graph's memory
+    return dgamma, dbeta, x.new_empty(n, dtype=torch.uint8) if n else None, n
 
 
 def layernorm_fwd(x: torch.Tensor, gamma=None, beta=None, eps: float = LN_EPS, act_slope: float = 1.0, p: float = 0.0,
@@ -900,12 +913,12 @@ def layernorm_fwd(x: torch.Tensor, gamma=None, beta=None, eps: float = LN_EPS, a
     if residual is not None:
         d.ld_res = _row_operand(residual, "residual", x)
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = _fresh(x)
         d.ld_out = d.cols
     else:
         d.ld_out = _row_operand(out, "out", x)
-    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    rstd = torch.empty_like(mean)
     check(L.load().fcd_layernorm_fwd(C.byref(d), x.data_ptr(), ptr(gamma), ptr(beta), ptr(residual), out.data_ptr(),
                                      mean.data_ptr(), rstd.data_ptr(), stream()), "layernorm_fwd")
     return out, mean, rstd
@@ -920,11 +933,11 @@ def layernorm_bwd(gy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: t
     d = _ln_desc(x, gamma, beta, 0.0, act_slope, p, rng)
     d.ld_gy = _row_operand(gy, "gy", x)
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = _fresh(x)
         d.ld_out = d.cols
     else:
         d.ld_out = _row_operand(out, "out", x)
-    dgamma, dbeta, ws, wn = _ln_affine(gamma, beta, want_affine, dgamma, dbeta, accumulate, d, x)
+    dgamma, dbeta, ws, wn = _ln_affine(gamma, beta, want_affine, dgamma, dbeta, accumulate, d, x, 0)
     check(L.load().fcd_layernorm_bwd(C.byref(d), gy.data_ptr(), x.data_ptr(), _ln_stat(mean, "mean", d, x),
                                      _ln_stat(rstd, "rstd", d, x), ptr(gamma), ptr(beta), out.data_ptr(), ptr(dgamma),
                                      ptr(dbeta), int(accumulate), ptr(ws), wn, stream()), "layernorm_bwd")
@@ -940,9 +953,8 @@ def layernorm_bwd2(ggx: torch.Tensor, gy: torch.Tensor, x: torch.Tensor, mean: t
     d.ld_gy = _row_operand(gy, "gy", x)
     d.ld_ggx = _row_operand(ggx, "ggx", x)
     d.ld_out = d.ld_ggy = d.cols
-    ggy = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    gx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    dgamma, dbeta, ws, wn = _ln_affine(gamma, beta, want_affine, dgamma, dbeta, accumulate, d, x)
+    ggy, gx = _fresh(x), _fresh(x)
+    dgamma, dbeta, ws, wn = _ln_affine(gamma, beta, want_affine, dgamma, dbeta, accumulate, d, x, 1)
     check(L.load().fcd_layernorm_bwd2(C.byref(d), ggx.data_ptr(), gy.data_ptr(), x.data_ptr(), _ln_stat(mean, "mean", d, x),
                                       _ln_stat(rstd, "rstd", d, x), ptr(gamma), ptr(beta), ggy.data_ptr(), gx.data_ptr(),
                                       ptr(dgamma), ptr(dbeta), int(accumulate), ptr(ws), wn, stream()), "layernorm_bwd2")

@@ -519,8 +519,9 @@ int fcd_layernorm_desc_bytes(void);
  * both be NULL. */
 int fcd_layernorm_fwd(const FcdLayerNormDesc* d, const void* x, const void* gamma, const void* beta,
                       const void* residual, void* y, float* mean, float* rstd, void* stream);
-/* Scratch of fcd_layernorm_bwd / _bwd2 when they compute dgamma / dbeta (0 without them). */
-size_t fcd_layernorm_workspace_bytes(const FcdLayerNormDesc* d);
+/* Scratch of fcd_layernorm_bwd (second 0) / _bwd2 (second 1) when they compute dgamma / dbeta (none without them); 0: none
+ * is needed, NULL will do. */
+size_t fcd_layernorm_workspace_bytes(const FcdLayerNormDesc* d, int second);
 /* With u = xhat * gamma + beta, g1 = drop(gy) * act'(u), a = g1 * gamma:
  *   dx = rstd * (a - mean(a) - xhat * mean(a * xhat)),  dgamma (+)= sum_rows g1 * xhat,  dbeta (+)= sum_rows g1.
  * (residual's gradient is gy itself.)  dgamma / dbeta NULL: not computed.  Row sums in a fixed order, no atomics. */

@@ -114,8 +114,8 @@ def test_forward_operands_refused():
 def test_backward_operands_refused():
     from fcd_amd import _lib
     lib = _lib.load()
-    d = desc()
-    need = lib.fcd_layernorm_workspace_bytes(C.byref(d))
+    d = desc(rows=400)
+    need = lib.fcd_layernorm_workspace_bytes(C.byref(d), 0)
     assert need >= 2 * 16 * 4
     f = lambda i: P * i
     call = lambda **k: lib.fcd_layernorm_bwd(C.byref(d), *[{**dict(gy=f(1), x=f(2), mean=f(3), rstd=f(4), ga=None, be=None, dx=f(5),
@@ -133,8 +133,10 @@ def test_backward_operands_refused():
     refused(d2(f(1), f(2), f(3), f(4), f(5), None, None, f(6), f(1) + 8, None, None, 0, None, 0, None), "overlaps ggx")
     refused(d2(None, f(2), f(3), f(4), f(5), None, None, f(6), f(7), None, None, 0, None, 0, None), "ggx is NULL")
     refused(d2(f(1), f(2), f(3), f(4), f(5), None, None, f(6), f(7), f(8), None, 0, f(9), 8, None), "workspace", -2)
-    assert lib.fcd_layernorm_workspace_bytes(None) == 0
-    assert lib.fcd_layernorm_workspace_bytes(C.byref(desc(rows=0))) == 0
+    for second in (0, 1):
+        assert lib.fcd_layernorm_workspace_bytes(None, second) == 0
+        assert lib.fcd_layernorm_workspace_bytes(C.byref(desc(rows=0)), second) == 0
+    assert lib.fcd_layernorm_workspace_bytes(C.byref(desc(rows=4)), 1) >= 2 * 16 * 4
 
 
 def test_dropout_refused():
@@ -189,10 +191,10 @@ def test_python_operands_refused():
         ops._row_operand(torch.zeros(4, 16, dtype=torch.float16), "gy", x)
     for p in (-0.1, 1.5, float("nan")):
         with pytest.raises(RuntimeError, match="probability"):
-            ops._rng_words(p, (1, 2), x.device)
+            ops._rng_words(p, (1, 2), 0)
     with pytest.raises(RuntimeError, match="needs rng"):
-        ops._rng_words(0.5, None, x.device)
+        ops._rng_words(0.5, None, 0)
     with pytest.raises(RuntimeError, match="int64"):
-        ops._rng_words(0.5, torch.zeros(2), x.device)
-    assert ops._rng_words(0.5, (-1, 2), x.device) == (2 ** 64 - 1, 2, None)
+        ops._rng_words(0.5, torch.zeros(2), 0)
+    assert ops._rng_words(0.5, (-1, 2), 0) == (2 ** 64 - 1, 2, None)
     assert ops.dropout_state(-5, "cpu", offset=(1 << 64) - 1).tolist() == [-5, -1]
