@@ -7,3 +7,4 @@ There is no CPU fallback: everything here launches into ``libfcd_hip.so``.
 from .generator import Generator, ResidualBlock  # noqa: F401
 from .discriminator import Discriminator  # noqa: F401
 from .solver import FCDSolver, FusedAdam, default_config  # noqa: F401
+from .layers import Dropout, LayerNorm  # noqa: F401

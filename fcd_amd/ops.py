@@ -801,10 +801,13 @@ def _rng_words(p: float, rng, device: int):
         return 0, 0, None
     if rng is None:
         raise RuntimeError("fcd_amd: dropout needs rng: (seed, offset) or what dropout_take returned")
+    extra = 0
+    if not isinstance(rng, torch.Tensor) and isinstance(rng[0], torch.Tensor):
+        rng, extra = rng[0], int(rng[1]) & _U64
     if isinstance(rng, torch.Tensor):
         if rng.dtype != torch.int64 or rng.numel() != 2 or not rng.is_contiguous() or rng.get_device() != device:
             raise RuntimeError("fcd_amd: a dropout rng tensor is two contiguous int64 words on the operands' device")
-        return 0, 0, rng.data_ptr()
+        return 0, extra, rng.data_ptr()
     seed, offset = rng
     return int(seed) & _U64, int(offset) & _U64, None
 
@@ -835,8 +838,8 @@ def dropout_take(state: torch.Tensor, numel: int) -> torch.Tensor:
 def dropout(x: torch.Tensor, p: float, rng, residual: Optional[torch.Tensor] = None,
             out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x * mask / (1 - p) (+ residual)``; the mask is a function of ``rng`` and the element's row-major index and is never
-    stored: the backward pass is the same call on the gradient (without ``residual``).  ``rng`` is ``(seed, offset)`` or
-    what :func:`dropout_take` returned; ``numel`` elements use ``ceil(numel / 8)`` offsets.  ``p`` is resolved to 2^-16.
+    stored: the backward pass is the same call on the gradient (without ``residual``).  ``rng`` is ``(seed, offset)``, what
+    :func:`dropout_take` returned, or ``(taken, offset to add)``; ``numel`` elements use ``ceil(numel / 8)`` offsets.  ``p`` is resolved to 2^-16.
     float32, bfloat16, float16; rows may be strided; ``out`` may be ``x``."""
     dt = _here(x, "x")
     rows, cols, ld = _rows(x, "x")
@@ -946,14 +949,19 @@ def layernorm_bwd(gy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: t
 
 def layernorm_bwd2(ggx: torch.Tensor, gy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, gamma=None,
                    beta=None, act_slope: float = 1.0, p: float = 0.0, rng=None, want_affine: bool = True, dgamma=None,
-                   dbeta=None, accumulate: bool = False):
+                   dbeta=None, accumulate: bool = False, outs=None):
     """Backward of :func:`layernorm_bwd`'s ``dx`` for its cotangent ``ggx`` (what a gradient penalty needs):
-    ``(ggy, gx, dgamma, dbeta)``, the cotangents of ``gy`` and ``x`` and the parameters' gradients."""
+    ``(ggy, gx, dgamma, dbeta)``, the cotangents of ``gy`` and ``x`` and the parameters' gradients.  ``outs``: tensors to
+    write ``(ggy, gx)`` into."""
     d = _ln_desc(x, gamma, beta, 0.0, act_slope, p, rng)
     d.ld_gy = _row_operand(gy, "gy", x)
     d.ld_ggx = _row_operand(ggx, "ggx", x)
-    d.ld_out = d.ld_ggy = d.cols
-    ggy, gx = _fresh(x), _fresh(x)
+    if outs is None:
+        ggy, gx = _fresh(x), _fresh(x)
+        d.ld_out = d.ld_ggy = d.cols
+    else:
+        ggy, gx = outs
+        d.ld_ggy, d.ld_out = _row_operand(ggy, "ggy", x), _row_operand(gx, "gx", x)
     dgamma, dbeta, ws, wn = _ln_affine(gamma, beta, want_affine, dgamma, dbeta, accumulate, d, x, 1)
     check(L.load().fcd_layernorm_bwd2(C.byref(d), ggx.data_ptr(), gy.data_ptr(), x.data_ptr(), _ln_stat(mean, "mean", d, x),
                                       _ln_stat(rstd, "rstd", d, x), ptr(gamma), ptr(beta), ggy.data_ptr(), gx.data_ptr(),

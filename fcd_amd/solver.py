@@ -34,7 +34,7 @@ def default_config(**over) -> Namespace:
                dataset="L8Biome", batch_size=16, num_iters=200000, num_iters_decay=100000, g_lr=1e-4, d_lr=1e-4,
                n_critic=5, beta1=0.5, beta2=0.999, act_D="lrelu", act_G="relu", n_feat_layers=4,
                interm_non_act=False, use_attention=False, use_feats=False, use_vgg=False, init_type="none",
-               num_channels=10, mode="train", precision="fp32", device="cuda")
+               num_channels=10, mode="train", precision="fp32", device="cuda", norm_D="none", dropout_D=0.0)
     cfg.update(over)
     return Namespace(**cfg)
 
@@ -214,7 +214,8 @@ class FCDSolver(nn.Module):
         self.G = Generator(self.g_conv_dim, self.c_dim, self.g_repeat_num, self.num_channels, activation=self.act_G)
         self.D = Discriminator(self.image_size, self.d_conv_dim, self.c_dim, self.d_repeat_num, self.num_channels,
                                activation=self.act_D, n_feature_layers=self.n_feature_layers,
-                               interm_non_act=self.interm_non_act)
+                               interm_non_act=self.interm_non_act, norm=getattr(self.config, "norm_D", "none"),
+                               dropout=float(getattr(self.config, "dropout_D", 0.0)))
 
     def set_precision(self, precision: str):
         """'fp32': exact-fp32 MFMA (v_mfma_f32_32x32x2_f32) everywhere.

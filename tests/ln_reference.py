@@ -136,7 +136,7 @@ def forward(x, gamma, beta, eps, code, mask, residual):
 
 
 def parts(x, gy, mean, rstd, gamma, beta, code, mask):
-    """What both backward passes share, given the statistics the forward pass left (exact operands here)."""
+    """What both backward passes share, given the statistics the forward pass left: exact operands, or Vs."""
     xh = (V(x) - mean) * rstd
     u = xh * gamma + beta
     g = V(gy) * V(mask, U * mask) if mask is not None else V(gy)

@@ -198,3 +198,30 @@ def test_python_operands_refused():
         ops._rng_words(0.5, torch.zeros(2), 0)
     assert ops._rng_words(0.5, (-1, 2), 0) == (2 ** 64 - 1, 2, None)
     assert ops.dropout_state(-5, "cpu", offset=(1 << 64) - 1).tolist() == [-5, -1]
+
+
+def test_critic_keys_and_refusals():
+    from fcd_amd import Discriminator
+    D = Discriminator(32, 8, 1, 3, 10, n_feature_layers=2, norm="layer", dropout=0.1, dropout_seed=3)
+    keys = set(D.state_dict())
+    assert {"features.0.0.weight", "features.0.1.weight", "features.0.1.bias", "main.0.1.weight", "dropout_state"} <= keys
+    assert "features.0.1.weight" not in Discriminator(32, 8, 1, 3, 10).state_dict()
+    with pytest.raises(NotImplementedError):
+        Discriminator(32, 8, 1, 3, 10, norm="batch")
+    with pytest.raises(NotImplementedError):
+        Discriminator(32, 8, 1, 3, 10, norm="layer", interm_non_act=True)
+    with pytest.raises(ValueError):
+        Discriminator(32, 8, 1, 3, 10, dropout=-0.5)
+
+
+def test_modules_refuse_the_cpu_and_bad_arguments():
+    from fcd_amd import Dropout, LayerNorm
+    with pytest.raises(RuntimeError, match="GPU"):
+        LayerNorm(8)(torch.zeros(2, 8))
+    with pytest.raises(RuntimeError, match="GPU"):
+        Dropout(0.5)(torch.zeros(2, 8))
+    assert Dropout(0.5).eval()(torch.zeros(2, 8)).shape == (2, 8)      # the identity launches nothing
+    with pytest.raises(ValueError):
+        Dropout(-0.1)
+    with pytest.raises(NotImplementedError):
+        LayerNorm(8, activation="tanh")
