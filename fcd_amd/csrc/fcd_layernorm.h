@@ -83,6 +83,19 @@ __device__ __forceinline__ void widen(const typename Oct<T>::type& o, float (&v)
   for (int j = 0; j < 8; ++j) v[j] = (float)o[j];
 }
 
+// Waits here for the load into `o`.  Loads and stores retire in one order, and whether a store was issued depends on the lane:
+// a wait for a prefetch that stands behind a row's stores is a wait for the stores as well.  So the next row's loads are
+// waited for in front of them.
+template <typename V>
+__device__ __forceinline__ void arrive(V& o) {
+  typedef int Quad __attribute__((ext_vector_type(4)));
+  struct Quads { Quad q[sizeof(V) / 16]; };
+  Quads t = __builtin_bit_cast(Quads, o);
+#pragma unroll
+  for (unsigned i = 0; i < sizeof(V) / 16; ++i) asm volatile("" : "+v"(t.q[i]));
+  o = __builtin_bit_cast(V, t);
+}
+
 // ---------------------------------------------------------------- sums -----------------
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v) {

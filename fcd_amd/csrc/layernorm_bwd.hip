@@ -95,9 +95,14 @@ __device__ __forceinline__ void bwd_rows(LnArgs p, unsigned blocks) {
     T* out = (T*)p.out + row * p.ld_out;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int c = (lane + k * G) * 8, n = G >= 64 || row < p.rows ? cols - c : 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) a[k][j] = fmaf(a[k][j], rstd, fmaf(xh[k][j], c1, c0));
+      arrive(nx[k]);
+      arrive(ng[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (lane + k * G) * 8, n = G >= 64 || row < p.rows ? cols - c : 0;
       store8(out + c, n, a[k]);
     }
   }

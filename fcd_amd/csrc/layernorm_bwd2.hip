@@ -140,6 +140,9 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd2_rows(LnArgs p) {
         }
       }
       if (EPI && p.drop.t) drop_apply(p.drop, w[k], gg);
+      arrive(nx[k]);
+      arrive(ng[k]);
+      arrive(nv[k]);
       if (n >= 8) {
         typename Oct<T>::type o, r;
 #pragma unroll

@@ -69,6 +69,8 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_fwd_rows(LnArgs p) {
     }
     T* out = (T*)p.out + row * p.ld_out;
 #pragma unroll
+    for (int k = 0; k < NV; ++k) arrive(nx[k]);
+#pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int c = (lane + k * G) * 8, n = here ? cols - c : 0;
       float u[8];
