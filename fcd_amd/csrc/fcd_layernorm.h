@@ -66,14 +66,29 @@ __device__ __forceinline__ void load_param(const void* p, int f32, N c, N n, flo
   }
 }
 
-// 8 elements as they are in memory; the ones past n are 0
-template <typename T, typename N>
-__device__ __forceinline__ void load_raw(const T* p, N n, typename Oct<T>::type& o) {
-  if (n >= 8) {
-    o = *reinterpret_cast<const typename Oct<T>::type*>(p);
-  } else {
+// A lane's unit of a row, prefetched: its 8 elements, or at a ragged end the row's last 8, which settle() moves down when they
+// are used.  (Lane by lane loads of an end would have to be waited for where they are issued.)  G = 4 may meet rows of less
+// than 8, whose elements are loaded one by one.
+template <typename T, int G>
+__device__ __forceinline__ void fetch8(const T* row, int c, int cols, typename Oct<T>::type& o) {
+  if (G == 4 && cols < 8) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = j < n ? p[j] : (T)0.f;
+    for (int j = 0; j < 8; ++j) o[j] = j < cols - c ? row[c + j] : (T)0.f;
+  } else {
+    o = *reinterpret_cast<const typename Oct<T>::type*>(row + (c < cols - 8 ? c : cols - 8));
+  }
+}
+
+// n: how many of the 8 exist (0 or less: none, all zero)
+template <typename T, int G>
+__device__ __forceinline__ void settle(typename Oct<T>::type& o, int cols, int n) {
+  if (n < 8 && !(G == 4 && cols < 8 && n > 0)) {
+    const typename Oct<T>::type z = {};
+    const int d = 8 - n;
+    typename Oct<T>::type r = d & 4 ? __builtin_shufflevector(o, z, 4, 5, 6, 7, 8, 8, 8, 8) : o;
+    r = d & 2 ? __builtin_shufflevector(r, z, 2, 3, 4, 5, 6, 7, 8, 8) : r;
+    r = d & 1 ? __builtin_shufflevector(r, z, 1, 2, 3, 4, 5, 6, 7, 8) : r;
+    o = n > 0 ? r : z;
   }
 }
 
@@ -86,14 +101,14 @@ __device__ __forceinline__ void widen(const typename Oct<T>::type& o, float (&v)
 // Waits here for the load into `o`.  Loads and stores retire in one order, and whether a store was issued depends on the lane:
 // a wait for a prefetch that stands behind a row's stores is a wait for the stores as well.  So the next row's loads are
 // waited for in front of them.
-template <typename V>
-__device__ __forceinline__ void arrive(V& o) {
+template <typename T>
+__device__ __forceinline__ void arrive(typename Oct<T>::type& o) {
   typedef int Quad __attribute__((ext_vector_type(4)));
-  struct Quads { Quad q[sizeof(V) / 16]; };
+  struct Quads { Quad q[sizeof(T) / 2]; };
   Quads t = __builtin_bit_cast(Quads, o);
 #pragma unroll
-  for (unsigned i = 0; i < sizeof(V) / 16; ++i) asm volatile("" : "+v"(t.q[i]));
-  o = __builtin_bit_cast(V, t);
+  for (unsigned i = 0; i < sizeof(T) / 2; ++i) asm volatile("" : "+v"(t.q[i]));
+  o = __builtin_bit_cast(typename Oct<T>::type, t);
 }
 
 // ---------------------------------------------------------------- sums -----------------

@@ -33,13 +33,10 @@ __device__ __forceinline__ void bwd_rows(LnArgs p, unsigned blocks) {
     const T *x = (const T*)p.x + r * p.ld_x, *gy = (const T*)p.gy + r * p.ld_gy;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int c = (lane + k * G) * 8, n = here ? cols - c : 0;
-      if (n >= 8) {
-        nx[k] = *(const typename Oct<T>::type*)(x + c);
-        ng[k] = *(const typename Oct<T>::type*)(gy + c);
-      } else {
-        load_raw<T>(x + c, n, nx[k]);
-        load_raw<T>(gy + c, n, ng[k]);
+      const int c = (lane + k * G) * 8;
+      if (here) {
+        fetch8<T, G>(x, c, cols, nx[k]);
+        fetch8<T, G>(gy, c, cols, ng[k]);
       }
     }
   };
@@ -48,11 +45,19 @@ __device__ __forceinline__ void bwd_rows(LnArgs p, unsigned blocks) {
   const long step = (long)blocks * RPB;
   const long turns = (p.rows - (G >= 64 ? row : (long)blockIdx.x * RPB) + step - 1) / step;
   if (turns > 0) fetch(row);
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    arrive<T>(nx[k]);
+    arrive<T>(ng[k]);
+  }
   for (long it = 0; it < turns; ++it, row += step) {
     const float mean = nmean, rstd = nrstd;
     float xh[NV][8], a[NV][8];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
+      const int n = G >= 64 || row < p.rows ? cols - (lane + k * G) * 8 : 0;
+      settle<T, G>(nx[k], cols, n);
+      settle<T, G>(ng[k], cols, n);
       widen<T>(nx[k], xh[k]);
       widen<T>(ng[k], a[k]);
     }
@@ -97,8 +102,8 @@ __device__ __forceinline__ void bwd_rows(LnArgs p, unsigned blocks) {
     for (int k = 0; k < NV; ++k) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) a[k][j] = fmaf(a[k][j], rstd, fmaf(xh[k][j], c1, c0));
-      arrive(nx[k]);
-      arrive(ng[k]);
+      arrive<T>(nx[k]);
+      arrive<T>(ng[k]);
     }
 #pragma unroll
     for (int k = 0; k < NV; ++k) {

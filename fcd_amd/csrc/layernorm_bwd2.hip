@@ -34,15 +34,11 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd2_rows(LnArgs p) {
     const T *x = (const T*)p.x + r * p.ld_x, *gy = (const T*)p.gy + r * p.ld_gy, *v = (const T*)p.ggx + r * p.ld_ggx;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int c = (lane + k * G) * 8, n = here ? cols - c : 0;
-      if (n >= 8) {
-        nx[k] = *(const typename Oct<T>::type*)(x + c);
-        ng[k] = *(const typename Oct<T>::type*)(gy + c);
-        nv[k] = *(const typename Oct<T>::type*)(v + c);
-      } else {
-        load_raw<T>(x + c, n, nx[k]);
-        load_raw<T>(gy + c, n, ng[k]);
-        load_raw<T>(v + c, n, nv[k]);
+      const int c = (lane + k * G) * 8;
+      if (here) {
+        fetch8<T, G>(x, c, cols, nx[k]);
+        fetch8<T, G>(gy, c, cols, ng[k]);
+        fetch8<T, G>(v, c, cols, nv[k]);
       }
     }
   };
@@ -50,19 +46,34 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd2_rows(LnArgs p) {
   long row = first_row<G, TH>();
   const long step = (long)gridDim.x * RPB;
   const long turns = (p.rows - (G >= 64 ? row : (long)blockIdx.x * RPB) + step - 1) / step;
-  if (turns > 0) fetch(row);
+  // a workgroup of 1024 has 128 registers a thread: behind an activation they do not hold the next row as well
+  constexpr bool AHEAD = !(G == 1024 && EPI == 2);
+  if (AHEAD && turns > 0) fetch(row);
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    if (AHEAD) {
+      arrive<T>(nx[k]);
+      arrive<T>(ng[k]);
+      arrive<T>(nv[k]);
+    }
+  }
   for (long it = 0; it < turns; ++it, row += step) {
+    if (!AHEAD) fetch(row);
     const float mean = nmean, rstd = nrstd;
     // xhat, drop(gy), v, and behind an activation act'(u) and act''(u)
     float xh[NV][8], g[NV][8], v[NV][8], d1[NV][8], q[NV][8], s[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
     uint32_t w[NV][4];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
+      const int n = G >= 64 || row < p.rows ? cols - (lane + k * G) * 8 : 0;
+      settle<T, G>(nx[k], cols, n);
+      settle<T, G>(ng[k], cols, n);
+      settle<T, G>(nv[k], cols, n);
       widen<T>(nx[k], xh[k]);
       widen<T>(ng[k], g[k]);
       widen<T>(nv[k], v[k]);
     }
-    if (it + 1 < turns) fetch(row + step);
+    if (AHEAD && it + 1 < turns) fetch(row + step);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       if (EPI && p.drop.t) {
@@ -140,9 +151,11 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd2_rows(LnArgs p) {
         }
       }
       if (EPI && p.drop.t) drop_apply(p.drop, w[k], gg);
-      arrive(nx[k]);
-      arrive(ng[k]);
-      arrive(nv[k]);
+      if (AHEAD) {
+        arrive<T>(nx[k]);
+        arrive<T>(ng[k]);
+        arrive<T>(nv[k]);
+      }
       if (n >= 8) {
         typename Oct<T>::type o, r;
 #pragma unroll

@@ -27,7 +27,7 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_fwd_rows(LnArgs p) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int c = (lane + k * G) * 8;
-      load_raw<T>(x + c, G >= 64 || r < p.rows ? cols - c : 0, o[k]);
+      if (G >= 64 || r < p.rows) fetch8<T, G>(x, c, cols, o[k]);
     }
   };
   // G < 64: every thread of a wave makes the same number of turns, for the sums need whole groups; G >= 64: whole waves do
@@ -35,11 +35,18 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_fwd_rows(LnArgs p) {
   const long step = (long)gridDim.x * RPB;
   const long turns = (p.rows - (G >= 64 ? row : (long)blockIdx.x * RPB) + step - 1) / step;
   if (turns > 0) fetch(p.x, p.ld_x, row, nx);
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    arrive<T>(nx[k]);
+  }
   for (long it = 0; it < turns; ++it, row += step) {
     const bool here = G >= 64 || row < p.rows;
     float v[NV][8];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) widen<T>(nx[k], v[k]);
+    for (int k = 0; k < NV; ++k) {
+      settle<T, G>(nx[k], cols, here ? cols - (lane + k * G) * 8 : 0);
+      widen<T>(nx[k], v[k]);
+    }
     typename Oct<T>::type rs[NV];
     if (EPI && p.res) fetch(p.res, p.ld_res, row, rs);
     if (it + 1 < turns) fetch(p.x, p.ld_x, row + step, nx);
@@ -69,7 +76,7 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_fwd_rows(LnArgs p) {
     }
     T* out = (T*)p.out + row * p.ld_out;
 #pragma unroll
-    for (int k = 0; k < NV; ++k) arrive(nx[k]);
+    for (int k = 0; k < NV; ++k) arrive<T>(nx[k]);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int c = (lane + k * G) * 8, n = here ? cols - c : 0;
@@ -90,6 +97,7 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_fwd_rows(LnArgs p) {
         }
         if (p.res) {
           float r[8];
+          settle<T, G>(rs[k], cols, n);
           widen<T>(rs[k], r);
 #pragma unroll
           for (int j = 0; j < 8; ++j) u[j] += r[j];
