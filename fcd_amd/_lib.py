@@ -149,8 +149,8 @@ PROTOTYPES = {
     "fcd_valid_minmax": (_I, [_P, _P, C.c_size_t, _P, _P]),
     "fcd_threshold_hist": (_I, [_P, _P, C.c_size_t, _P, _I, _P, _P]),
     "fcd_layernorm_desc_bytes": (_I, []),
-    "fcd_layernorm_fwd": (_I, [C.POINTER(LayerNormDesc), _P, _P, _P, _P, _P, _P, _P, _P]),
-    "fcd_layernorm_workspace_bytes": (_Z, [C.POINTER(LayerNormDesc), _I]),
+    "fcd_layernorm_fwd": (_I, [C.POINTER(LayerNormDesc), _P, _P, _P, _P, _P, _P, _P, _P, _Z, _P]),
+    "fcd_layernorm_workspace_bytes": (_Z, [C.POINTER(LayerNormDesc), _I, _I]),
     "fcd_layernorm_bwd": (_I, [C.POINTER(LayerNormDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _Z, _P]),
     "fcd_layernorm_bwd2": (_I, [C.POINTER(LayerNormDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _Z, _P]),
     "fcd_dropout": (_I, [_P, _P, _P, _L, _L, _L, _L, _L, _I, C.c_double, _U, _U, _P, _P]),

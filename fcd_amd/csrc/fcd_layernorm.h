@@ -6,7 +6,8 @@ struct LnArgs {
   const void *x, *res, *gy, *ggx, *gamma, *beta;
   void *out, *ggy;
   float *mean, *rstd;      // written by fwd, read by bwd / bwd2
-  float* partial;          // [groups][2][cols]: a workgroup's sums of dgamma and dbeta; or NULL
+  float* partial;          // scratch, [groups][2][cols]: a workgroup's sums of dgamma and dbeta; or NULL
+  float *chunk, *row;      // scratch of rows that are split: [rows][chunks][K] sums and [rows][ROW_SUMS] joined ones
   long rows, cols, ld_x, ld_res, ld_gy, ld_ggx, ld_out, ld_ggy;
   float eps, act;
   int param_f32;
@@ -17,24 +18,24 @@ struct LnArgs {
 int ln_check(const char* who, const FcdLayerNormDesc* d, LnArgs* a);
 int ln_check_vectors(const char* who, const FcdLayerNormDesc* d, const void* gamma, const void* beta, const void* mean,
                      const void* rstd);
-int ln_check_affine(const char* who, const FcdLayerNormDesc* d, int second, const void* dgamma, const void* dbeta, void* workspace,
-                    size_t workspace_bytes, LnArgs* a);
+int ln_check_scratch(const char* who, const FcdLayerNormDesc* d, int pass, const void* dgamma, const void* dbeta, void* workspace,
+                     size_t workspace_bytes, LnArgs* a);
 int ln_finish(const char* who, const FcdLayerNormDesc* d, const LnArgs& a, int groups, void* dgamma, void* dbeta, int accumulate,
               hipStream_t st);
-int ln_groups(int64_t rows, int64_t cols);   // workgroups of the backward passes
+int ln_groups(int64_t rows, int64_t cols);   // workgroups (row groups of split rows) of the backward passes
 bool ln_few_rows(int64_t rows, int64_t cols);   // the first backward pass sums its columns beside the rows, in one launch
 
 // Where a row lives: G threads with NV units of 8 elements each.  G <= 64: the row's sums stay inside a wave, and a workgroup
-// of 256 works on 256 / G rows with no barrier; G > 64: one workgroup per row, one barrier per sum.  Longer rows than the last
-// shape takes are read again from cache for every pass (ln_*_long).  The forward pass keeps two units a thread (fewer waves
-// meet at the barrier); the backward passes hold the affine sums as well and keep one.
+// of 256 works on 256 / G rows with no barrier; G > 64: one workgroup per row, one barrier per sum.  The forward pass keeps
+// two units a thread (fewer waves meet at the barrier); the backward passes hold the affine sums as well and keep one.
+// Longer rows than the last shape takes are split (below).
 #define LN_FWD_SHAPES(F) \
   F(4, 1) F(8, 1) F(16, 1) F(32, 1) F(64, 1) F(64, 2) F(256, 1) F(256, 2) F(512, 2) F(1024, 2)
 #define LN_BWD_SHAPES(F) \
   F(4, 1) F(8, 1) F(16, 1) F(32, 1) F(64, 1) F(128, 1) F(256, 1) F(512, 1) F(1024, 1)
 
 struct LnShape {
-  int g, nv;   // g 0: the long form
+  int g, nv;   // g 0: split rows
 };
 
 static inline LnShape ln_bwd_shape(int64_t cols) {
@@ -45,6 +46,22 @@ static inline LnShape ln_bwd_shape(int64_t cols) {
 #undef PICK
   return {0, 0};
 }
+constexpr int64_t LN_FWD_MAX = 16384;   // the last forward shape's columns
+static_assert(LN_FWD_MAX >= FCD_LN_WHOLE, "");
+
+// Split rows: one kernel sums chunks of a row, one joins the chunks of every row, and one streams: its workgroups own 2048
+// columns, keep their parameters and affine sums in registers and walk down a group of rows whose sums are known, with no
+// barrier.  The operands are read once more than by the shapes above, which is what a row of any length and a few long rows
+// (one workgroup each would leave the card idle) cost.
+constexpr int CHUNK = 8192;             // columns of a chunk: 256 threads, 4 units each
+constexpr int ROW_SUMS = 7;
+static inline int64_t ln_chunks(int64_t cols) { return (cols + CHUNK - 1) / CHUNK; }
+static inline unsigned ln_items(int64_t rows, int64_t cols) {
+  const __int128 n = (__int128)rows * ln_chunks(cols);
+  return (unsigned)(n < 16384 ? n : 16384);
+}
+static inline dim3 ln_stream_grid(int64_t rows, int64_t cols) { return dim3((unsigned)((cols + 2047) / 2048), ln_groups(rows, cols)); }
+static inline unsigned ln_join_grid(int64_t rows) { return (unsigned)(rows < 65536 ? (rows + 3) / 4 : 16384); }
 
 // The row of a thread (wave-uniform where it can be, so that row addresses live in scalar registers) and its first column.
 template <int G, int TH>
@@ -239,44 +256,29 @@ __device__ __forceinline__ void ln_act8(const float (&u)[8], float code, float* 
 }
 
 // ---------------------------------------------------------------- backward passes ------
-// Long rows: what the backward passes need of 8 elements: xhat, drop(gy), g1 = drop(gy) act'(u), a = g1 gamma; elements past
-// the row's end: 0.
+// What the backward passes need of 8 elements of x and gy: xhat, drop(gy), and behind an activation act'(u), act''(u).
+// Absent elements (gy 0) come out with drop(gy) = 0.
+template <int EPI, bool SECOND>
 struct Eight {
-  float xh[8], gy[8], ga[8], g1[8], a[8], d1[8], d2[8];
+  float xh[8], g[8], d1[8], d2[8];
   uint32_t w[4];
+
+  __device__ __forceinline__ void make(const LnArgs& p, long row, int c, float mean, float rstd, const float (&ga)[8],
+                                       const float (&be)[8]) {
+    if (EPI && p.drop.t) {
+      drop_draw8(p.drop, (uint64_t)(row * p.cols + c), w);
+      drop_apply(p.drop, w, g);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) xh[j] = (xh[j] - mean) * rstd;
+    if (EPI == 2) {
+      float u[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) u[j] = fmaf(xh[j], ga[j], be[j]);
+      ln_act8(u, p.act, nullptr, d1, SECOND ? d2 : nullptr);
+    }
+  }
 };
-
-template <typename T, bool SECOND>
-__device__ __forceinline__ void load_eight(const LnArgs& p, long row, long c, float mean, float rstd, Eight& e) {
-  const long n = p.cols - c;
-  float be[8], u[8];
-  load8((const T*)p.x + row * p.ld_x + c, n, e.xh);
-  load8((const T*)p.gy + row * p.ld_gy + c, n, e.gy);
-  load_param<T>(p.gamma, p.param_f32, c, n, 1.f, e.ga);
-  load_param<T>(p.beta, p.param_f32, c, n, 0.f, be);
-  if (p.drop.t) {
-    drop_draw8(p.drop, (uint64_t)(row * p.cols + c), e.w);
-    drop_apply(p.drop, e.w, e.gy);
-  }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    e.xh[j] = j < n ? (e.xh[j] - mean) * rstd : 0.f;
-    u[j] = fmaf(e.xh[j], e.ga[j], be[j]);
-  }
-  ln_act8(u, p.act, nullptr, e.d1, SECOND ? e.d2 : nullptr);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    e.g1[j] = j < n ? e.gy[j] * e.d1[j] : 0.f;
-    e.a[j] = e.g1[j] * e.ga[j];
-  }
-}
-
-// Adds to this workgroup's sums; a thread meets the same columns in every row, so nothing else touches them.
-__device__ __forceinline__ void add_partial(float* p, long n, bool first, const float (&v)[8]) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (j < n) p[j] = first ? v[j] : p[j] + v[j];
-}
 
 // Affine sums of a workgroup whose threads each kept NV * 8 columns in registers: over the groups of a wave by exchanges, over
 // the waves through LDS, in a fixed order; then to the workgroup's place in the scratch.
@@ -316,6 +318,25 @@ __device__ __forceinline__ void write_partial(const LnArgs& p, float (&dg)[NV][8
     for (int i = threadIdx.x; i < 2 * W; i += 256) {
       const int which = i / W, c = i % W;
       if (c < cols) part[which * cols + c] = (sm[i] + sm[2 * W + i]) + (sm[4 * W + i] + sm[6 * W + i]);
+    }
+  }
+}
+
+// Sums of a row's chunks, joined by a wave.
+template <int K>
+__global__ __launch_bounds__(256) void ln_join(const float* chunk, long rows, long chunks, float* row_sums, int first) {
+  const int lane = threadIdx.x & 63;
+  for (long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6); row < rows; row += (long)gridDim.x * 4) {
+    float s[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) s[k] = 0.f;
+    for (long i = lane; i < chunks; i += 64)
+#pragma unroll
+      for (int k = 0; k < K; ++k) s[k] += chunk[(row * chunks + i) * K + k];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      s[k] = lanes_sum<64>(s[k]);
+      if (lane == 0) row_sums[row * ROW_SUMS + first + k] = s[k];
     }
   }
 }

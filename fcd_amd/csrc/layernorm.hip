@@ -3,33 +3,36 @@
 
 namespace {
 
-// dgamma (blockIdx.y 0) / dbeta (1): the workgroups' sums of 16 columns, 32 strands of them added in order and then joined.
+// dgamma (blockIdx.y 0) / dbeta (1): the workgroups' sums of a column, added in 2^ls strands and joined in order.  Up to 32
+// strands of 16 columns (64-byte accesses) where there are many sums, down to one strand of 512 columns.
 template <typename P>
-__global__ __launch_bounds__(512) void ln_affine_reduce(const float* partial, int groups, long cols, P* dgamma, P* dbeta,
+__global__ __launch_bounds__(512) void ln_affine_reduce(const float* partial, int groups, long cols, int ls, P* dgamma, P* dbeta,
                                                         int accumulate) {
-  __shared__ float sm[32][17];
+  __shared__ float sm[512];
   P* out = blockIdx.y ? dbeta : dgamma;
   if (!out) return;
-  const int col = threadIdx.x & 15, strand = threadIdx.x >> 4;
-  const long c = (long)blockIdx.x * 16 + col;
+  const int strands = 1 << ls, width = 512 >> ls, col = threadIdx.x & (width - 1), strand = threadIdx.x >> (9 - ls);
+  const long c = (long)blockIdx.x * width + col;
   float s = 0.f;
   if (c < cols)
 #pragma unroll 4
-    for (int g = strand; g < groups; g += 32) s += partial[((long)g * 2 + blockIdx.y) * cols + c];
-  sm[strand][col] = s;
+    for (int g = strand; g < groups; g += strands) s += partial[((long)g * 2 + blockIdx.y) * cols + c];
+  sm[threadIdx.x] = s;
   __syncthreads();
   if (strand == 0 && c < cols) {
     s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) s += sm[i][col];
+    for (int i = 0; i < strands; ++i) s += sm[i * width + col];
     out[c] = (P)(accumulate ? (float)out[c] + s : s);
   }
 }
 
 template <typename P>
 int reduce(const char* who, const LnArgs& a, int groups, void* dgamma, void* dbeta, int accumulate, hipStream_t st) {
-  ln_affine_reduce<P><<<dim3((unsigned)((a.cols + 15) / 16), 2), 512, 0, st>>>(a.partial, groups, a.cols, (P*)dgamma, (P*)dbeta,
-                                                                               accumulate);
+  int ls = 0;
+  while (ls < 5 && (1 << ls) < groups) ++ls;
+  const long width = 512 >> ls;
+  ln_affine_reduce<P><<<dim3((unsigned)((a.cols + width - 1) / width), 2), 512, 0, st>>>(a.partial, groups, a.cols, ls, (P*)dgamma,
+                                                                                        (P*)dbeta, accumulate);
   return fcd_check_launch(who);
 }
 
@@ -44,7 +47,13 @@ static int64_t tune(const char* n, int64_t v) { const char* e = getenv(n); retur
 int ln_groups(int64_t rows, int64_t cols) {
   const LnShape s = ln_bwd_shape(cols);
   const int64_t rpb = s.g > 0 && s.g <= 64 ? 256 / s.g : 1, need = (rows + rpb - 1) / rpb;
-  const int64_t full = s.g <= 64 ? tune("LN_W", 512) : s.g == 0 ? 512 : 256 * (s.g >= tune("LN_B", 512) ? 1 : tune("LN_B", 512) / s.g);
+  int64_t full;
+  if (s.g == 0) {            // split rows: enough workgroups of 2048 columns for the card, and not more than 256 sums of a column
+    full = 2048 / ((cols + 2047) / 2048);
+    full = full < 1 ? 1 : full > 256 ? 256 : full;
+  } else {
+    full = s.g <= 64 ? tune("LN_W", 512) : 256 * (s.g >= tune("LN_B", 512) ? 1 : tune("LN_B", 512) / s.g);
+  }
   return (int)(need < full ? need : full);
 }
 
@@ -60,17 +69,44 @@ int ln_finish(const char* who, const FcdLayerNormDesc* d, const LnArgs& a, int g
   return reduce<f16_t>(who, a, groups, dgamma, dbeta, accumulate, st);
 }
 
-int ln_check_affine(const char* who, const FcdLayerNormDesc* d, int second, const void* dgamma, const void* dbeta, void* workspace,
-                    size_t workspace_bytes, LnArgs* a) {
+namespace {
+
+// Scratch of one pass, in floats from its start: affine sums, chunk sums, row sums.
+struct Scratch {
+  size_t chunk, row, bytes;
+};
+
+Scratch scratch(const FcdLayerNormDesc* d, int pass, bool affine) {
+  Scratch s = {};
+  if (d->rows <= 0 || d->cols <= 0) return s;
+  const size_t rows = (size_t)d->rows, cols = (size_t)d->cols;
+  const bool split = pass == FCD_LN_FWD ? d->cols > LN_FWD_MAX : ln_bwd_shape(d->cols).g == 0;
+  if (pass != FCD_LN_FWD && affine && !(pass == FCD_LN_BWD && ln_few_rows(d->rows, d->cols)))
+    s.chunk = (size_t)ln_groups(d->rows, d->cols) * 2 * cols;
+  s.row = s.chunk;
+  s.bytes = s.chunk * sizeof(float);
+  if (split) {
+    s.row += rows * (size_t)ln_chunks(d->cols) * (pass == FCD_LN_BWD2 ? 5 : 2);
+    s.bytes = (s.row + rows * (pass == FCD_LN_FWD ? 2 : ROW_SUMS)) * sizeof(float);
+  }
+  return s;
+}
+
+}  // namespace
+
+int ln_check_scratch(const char* who, const FcdLayerNormDesc* d, int pass, const void* dgamma, const void* dbeta, void* workspace,
+                     size_t workspace_bytes, LnArgs* a) {
   FCD_TRY(ln_check_vectors(who, d, dgamma, dbeta, nullptr, nullptr));
-  if (!dgamma && !dbeta) return FCD_OK;
-  const size_t need = fcd_layernorm_workspace_bytes(d, second);
-  if (workspace_bytes < need) {
-    fcd_set_error("%s: workspace of %zu bytes, needs %zu", who, workspace_bytes, need);
+  const bool affine = dgamma || dbeta;
+  const Scratch s = scratch(d, pass, affine);
+  if (workspace_bytes < s.bytes) {
+    fcd_set_error("%s: workspace of %zu bytes, needs %zu", who, workspace_bytes, s.bytes);
     return FCD_EWORKSPACE;
   }
-  FCD_REQUIRE(need == 0 || (workspace && ((uintptr_t)workspace & 15u) == 0), "%s: workspace is NULL or not 16-byte aligned", who);
-  a->partial = (float*)workspace;
+  FCD_REQUIRE(s.bytes == 0 || (workspace && ((uintptr_t)workspace & 15u) == 0), "%s: workspace is NULL or not 16-byte aligned", who);
+  if (s.chunk) a->partial = (float*)workspace;
+  a->chunk = (float*)workspace + s.chunk;
+  a->row = (float*)workspace + s.row;
   return FCD_OK;
 }
 
@@ -79,7 +115,7 @@ int ln_check(const char* who, const FcdLayerNormDesc* d, LnArgs* a) {
   FCD_REQUIRE(fcd_dt_bytes(d->dtype), "%s: unknown element type %d", who, d->dtype);
   FCD_REQUIRE(d->param_dtype == FCD_DT_F32 || d->param_dtype == d->dtype, "%s: parameters must be fp32 or of x's type", who);
   FCD_REQUIRE(d->rows >= 0, "%s: negative number of rows", who);
-  FCD_REQUIRE(d->cols >= 1 && d->cols < (int64_t)1 << 31, "%s: %lld columns (1 ... 2^31 - 1)", who, (long long)d->cols);
+  FCD_REQUIRE(d->cols >= 1 && d->cols <= (int64_t)1 << 30, "%s: %lld columns (1 ... 2^30)", who, (long long)d->cols);
   FCD_REQUIRE(d->rows < (int64_t)1 << 58 && (__int128)d->rows * d->cols < (__int128)1 << 58, "%s: too many elements", who);
   FCD_REQUIRE(d->eps >= 0.f && d->eps <= 3.4e38f, "%s: eps must be finite and not negative", who);
   FCD_REQUIRE((d->act >= 0.f && d->act <= 1.f) || d->act == FCD_ACT_SILU || d->act == FCD_ACT_MISH,
@@ -104,7 +140,6 @@ int ln_check_vectors(const char* who, const FcdLayerNormDesc* d, const void* gam
 
 extern "C" int fcd_layernorm_desc_bytes(void) { return (int)sizeof(FcdLayerNormDesc); }
 
-extern "C" size_t fcd_layernorm_workspace_bytes(const FcdLayerNormDesc* d, int second) {
-  if (!d || d->rows <= 0 || d->cols <= 0 || (!second && ln_few_rows(d->rows, d->cols))) return 0;
-  return (size_t)ln_groups(d->rows, d->cols) * 2 * (size_t)d->cols * sizeof(float);
+extern "C" size_t fcd_layernorm_workspace_bytes(const FcdLayerNormDesc* d, int pass, int affine) {
+  return d && pass >= FCD_LN_FWD && pass <= FCD_LN_BWD2 ? scratch(d, pass, affine != 0).bytes : 0;
 }

@@ -207,53 +207,111 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd_few(LnArgs p, Affine 
   }
 }
 
-// Rows too long for registers: both operands read again for every pass, the affine sums kept in the scratch.
-template <typename T>
-__global__ __launch_bounds__(1024) void ln_bwd_long(LnArgs p) {
-  constexpr int TH = 1024;
-  __shared__ float sm[2 * 2 * TH / 64];
+// Split rows, 1: a chunk's two sums.
+template <typename T, int EPI>
+__global__ __launch_bounds__(256) void ln_bwd_chunks(LnArgs p, long chunks) {
+  __shared__ float sm[2 * 2 * 4];
   int turn = 0;
-  drop_state(p.drop);
-  const float inv = 1.f / (float)p.cols;
-  for (long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+  if (EPI) drop_state(p.drop);
+  for (long item = blockIdx.x; item < p.rows * chunks; item += gridDim.x) {
+    const long row = item / chunks, c0 = (item - row * chunks) * CHUNK;
+    const T *x = (const T*)p.x + row * p.ld_x, *gy = (const T*)p.gy + row * p.ld_gy;
     const float mean = p.mean[row], rstd = p.rstd[row];
     float s[2] = {0.f, 0.f};
-    for (long c = threadIdx.x * 8; c < p.cols; c += TH * 8) {
-      Eight e;
-      load_eight<T, false>(p, row, c, mean, rstd, e);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int c = (int)c0 + (threadIdx.x + k * 256) * 8, n = (int)p.cols - c;
+      Eight<EPI, false> e;
+      float ga[8], be[8];
+      load8(x + c, n, e.xh);
+      load8(gy + c, n, e.g);
+      load_param<T>(p.gamma, p.param_f32, c, n, 1.f, ga);
+      if (EPI == 2) load_param<T>(p.beta, p.param_f32, c, n, 0.f, be);
+      e.make(p, row, c, mean, rstd, ga, be);
+      float s0 = 0.f, s1 = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        s[0] += e.a[j];
-        s[1] += e.a[j] * e.xh[j];
+        const float a = (EPI == 2 ? e.g[j] * e.d1[j] : e.g[j]) * ga[j];
+        s0 += a;
+        s1 = fmaf(a, e.xh[j], s1);
       }
+      s[0] += s0;
+      s[1] += s1;
     }
-    RowSums<TH, 2>::run(s, sm, turn);
-    const float am = s[0] * inv, ax = s[1] * inv;
-    for (long c = threadIdx.x * 8; c < p.cols; c += TH * 8) {
-      const long n = p.cols - c;
-      Eight e;
-      load_eight<T, false>(p, row, c, mean, rstd, e);
-      float dx[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) dx[j] = rstd * (e.a[j] - am - e.xh[j] * ax);
-      if (p.partial) {
-        float* part = p.partial + (long)blockIdx.x * 2 * p.cols + c;
-        float dg[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) dg[j] = e.g1[j] * e.xh[j];
-        add_partial(part, n, row == blockIdx.x, dg);
-        add_partial(part + p.cols, n, row == blockIdx.x, e.g1);
-      }
-      store8((T*)p.out + row * p.ld_out + c, n, dx);
+    RowSums<256, 2>::run(s, sm, turn);
+    if (threadIdx.x == 0) {
+      p.chunk[item * 2] = s[0];
+      p.chunk[item * 2 + 1] = s[1];
     }
   }
+}
+
+// 3 (2 is ln_join): dx and the affine sums of a row group.
+template <typename T, int EPI>
+__global__ __launch_bounds__(256) void ln_bwd_stream(LnArgs p) {
+  if (EPI) drop_state(p.drop);
+  const int c = (int)((blockIdx.x * 256u + threadIdx.x) * 8), cols = (int)p.cols, n = cols - c;
+  if (n <= 0) return;
+  const float inv = 1.f / (float)cols;
+  float ga[8], be[8], dg[8], db[8];
+  load_param<T>(p.gamma, p.param_f32, c, n, 1.f, ga);
+  if (EPI == 2) load_param<T>(p.beta, p.param_f32, c, n, 0.f, be);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) dg[j] = db[j] = 0.f;
+  typename Oct<T>::type nx, ng;
+  long row = blockIdx.y;
+  fetch8<T, 64>((const T*)p.x + row * p.ld_x, c, cols, nx);
+  fetch8<T, 64>((const T*)p.gy + row * p.ld_gy, c, cols, ng);
+  arrive<T>(nx);
+  arrive<T>(ng);
+  for (; row < p.rows; row += gridDim.y) {
+    settle<T, 64>(nx, cols, n);
+    settle<T, 64>(ng, cols, n);
+    Eight<EPI, false> e;
+    widen<T>(nx, e.xh);
+    widen<T>(ng, e.g);
+    const long next = row + gridDim.y;
+    if (next < p.rows) {
+      fetch8<T, 64>((const T*)p.x + next * p.ld_x, c, cols, nx);
+      fetch8<T, 64>((const T*)p.gy + next * p.ld_gy, c, cols, ng);
+    }
+    const float mean = p.mean[row], rstd = p.rstd[row];
+    const float c0 = -rstd * (p.row[row * ROW_SUMS] * inv), c1 = -rstd * (p.row[row * ROW_SUMS + 1] * inv);
+    e.make(p, row, c, mean, rstd, ga, be);
+    float dx[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float g1 = EPI == 2 ? e.g[j] * e.d1[j] : e.g[j];
+      dg[j] = fmaf(g1, e.xh[j], dg[j]);
+      db[j] += g1;
+      dx[j] = fmaf(g1 * ga[j], rstd, fmaf(e.xh[j], c1, c0));
+    }
+    arrive<T>(nx);
+    arrive<T>(ng);
+    store8((T*)p.out + row * p.ld_out + c, n, dx);
+  }
+  if (p.partial) {
+    float* part = p.partial + (long)blockIdx.y * 2 * cols + c;
+    store8(part, n, dg);
+    store8(part + cols, n, db);
+  }
+}
+
+template <typename T, int EPI>
+void launch_split(const LnArgs& a, hipStream_t st) {
+  const long chunks = ln_chunks(a.cols);
+  ln_bwd_chunks<T, EPI><<<ln_items(a.rows, a.cols), 256, 0, st>>>(a, chunks);
+  ln_join<2><<<ln_join_grid(a.rows), 256, 0, st>>>(a.chunk, a.rows, chunks, a.row, 0);
+  ln_bwd_stream<T, EPI><<<ln_stream_grid(a.rows, a.cols), 256, 0, st>>>(a);
 }
 
 template <typename T>
 void launch(const LnArgs& a, int groups, hipStream_t st) {
   const LnShape s = ln_bwd_shape(a.cols);
   if (s.g == 0) {
-    ln_bwd_long<T><<<groups, 1024, 0, st>>>(a);
+    if (a.act != 1.f) launch_split<T, 2>(a, st);
+    else if (a.drop.t) launch_split<T, 1>(a, st);
+    else launch_split<T, 0>(a, st);
     return;
   }
 #define SHAPE(G, NV)                                                                                      \
@@ -297,7 +355,7 @@ extern "C" int fcd_layernorm_bwd(const FcdLayerNormDesc* d, const void* gy, cons
   FCD_TRY(fcd_check_apart(who, vo, vg, d->rows, d->cols, es, true));
   FCD_TRY(ln_check_vectors(who, d, gamma, beta, mean, rstd));
   FCD_REQUIRE(d->rows == 0 || (mean && rstd), "%s: mean / rstd are NULL", who);
-  FCD_TRY(ln_check_affine(who, d, 0, dgamma, dbeta, workspace, workspace_bytes, &a));
+  FCD_TRY(ln_check_scratch(who, d, FCD_LN_BWD, dgamma, dbeta, workspace, workspace_bytes, &a));
   a.x = x, a.gy = gy, a.gamma = gamma, a.beta = beta, a.out = dx, a.mean = (float*)mean, a.rstd = (float*)rstd;
   const int groups = ln_groups(d->rows, d->cols);
   hipStream_t st = fcd_stream(stream);

@@ -171,86 +171,132 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd2_rows(LnArgs p) {
   if (p.partial) write_partial<G, NV>(p, dg, db, aff);
 }
 
-// Rows too long for registers: both operands read again for every pass, the affine sums kept in the scratch.
-template <typename T>
-__global__ __launch_bounds__(1024) void ln_bwd2_long(LnArgs p) {
-  constexpr int TH = 1024;
-  __shared__ float sm[2 * 5 * TH / 64];
-  int turn = 0, turn2 = 0;
-  __shared__ float sm2[2 * 2 * TH / 64];
-  drop_state(p.drop);
+// Split rows, 1: a chunk's five sums; with the joined ones known and a curved activation (CURVED) the two sums of q gamma.
+template <typename T, int EPI, bool CURVED>
+__global__ __launch_bounds__(256) void ln_bwd2_chunks(LnArgs p, long chunks) {
+  constexpr int K = CURVED ? 2 : 5;
+  __shared__ float sm[2 * K * 4];
+  int turn = 0;
+  if (EPI) drop_state(p.drop);
   const float inv = 1.f / (float)p.cols;
-  const bool smooth = p.act > 1.f;
-  for (long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+  for (long item = blockIdx.x; item < p.rows * chunks; item += gridDim.x) {
+    const long row = item / chunks, c0 = (item - row * chunks) * CHUNK;
+    const T *x = (const T*)p.x + row * p.ld_x, *gy = (const T*)p.gy + row * p.ld_gy, *ggx = (const T*)p.ggx + row * p.ld_ggx;
     const float mean = p.mean[row], rstd = p.rstd[row];
-    float s[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
-    for (long c = threadIdx.x * 8; c < p.cols; c += TH * 8) {
-      Eight e;
-      float v[8];
-      load_eight<T, true>(p, row, c, mean, rstd, e);
-      load8((const T*)p.ggx + row * p.ld_ggx + c, p.cols - c, v);
+    const float vm = CURVED ? p.row[row * ROW_SUMS + 2] * inv : 0.f, vx = CURVED ? p.row[row * ROW_SUMS + 3] * inv : 0.f;
+    float s[K];
+#pragma unroll
+    for (int i = 0; i < K; ++i) s[i] = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int c = (int)c0 + (threadIdx.x + k * 256) * 8, n = (int)p.cols - c;
+      Eight<EPI, CURVED> e;
+      float ga[8], be[8], v[8];
+      load8(x + c, n, e.xh);
+      load8(gy + c, n, e.g);
+      load8(ggx + c, n, v);
+      load_param<T>(p.gamma, p.param_f32, c, n, 1.f, ga);
+      if (EPI == 2) load_param<T>(p.beta, p.param_f32, c, n, 0.f, be);
+      e.make(p, row, c, mean, rstd, ga, be);
+      float t[K];
+#pragma unroll
+      for (int i = 0; i < K; ++i) t[i] = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        s[0] += e.a[j];
-        s[1] += e.a[j] * e.xh[j];
-        s[2] += v[j];
-        s[3] += v[j] * e.xh[j];
-        s[4] += v[j] * e.a[j];
-      }
-    }
-    RowSums<TH, 5>::run(s, sm, turn);
-    const float am = s[0] * inv, ax = s[1] * inv, vm = s[2] * inv, vx = s[3] * inv;
-    const float sv = s[4] * inv - vm * am - vx * ax;
-    float q2[2] = {0.f, 0.f};
-    if (smooth) {
-      for (long c = threadIdx.x * 8; c < p.cols; c += TH * 8) {
-        Eight e;
-        float v[8];
-        load_eight<T, true>(p, row, c, mean, rstd, e);
-        load8((const T*)p.ggx + row * p.ld_ggx + c, p.cols - c, v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float t = rstd * (v[j] - vm - e.xh[j] * vx);
-          const float qg = j < p.cols - c ? e.gy[j] * e.d2[j] * e.ga[j] * t * e.ga[j] : 0.f;
-          q2[0] += qg;
-          q2[1] += qg * e.xh[j];
+        if constexpr (CURVED) {
+          const float qg = e.g[j] * e.d2[j] * ga[j] * (rstd * (v[j] - vm - e.xh[j] * vx)) * ga[j];
+          t[0] += qg;
+          t[1] = fmaf(qg, e.xh[j], t[1]);
+        } else {
+          const float a = (EPI == 2 ? e.g[j] * e.d1[j] : e.g[j]) * ga[j];
+          t[0] += a;
+          t[1] = fmaf(a, e.xh[j], t[1]);
+          t[2] += v[j];
+          t[3] = fmaf(v[j], e.xh[j], t[3]);
+          t[4] = fmaf(v[j], a, t[4]);
         }
       }
-      RowSums<TH, 2>::run(q2, sm2, turn2);
-    }
-    const float hm = q2[0] * inv - rstd * (vm * ax + am * vx), hx = q2[1] * inv - 2.f * rstd * vx * ax;
-    for (long c = threadIdx.x * 8; c < p.cols; c += TH * 8) {
-      const long n = p.cols - c;
-      Eight e;
-      float v[8], gg[8], gx[8], dg[8], q[8];
-      load_eight<T, true>(p, row, c, mean, rstd, e);
-      load8((const T*)p.ggx + row * p.ld_ggx + c, n, v);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float t = rstd * (v[j] - vm - e.xh[j] * vx);
-        q[j] = smooth ? e.gy[j] * e.d2[j] * e.ga[j] * t : 0.f;
-        gg[j] = e.d1[j] * e.ga[j] * t;
-        const float h = q[j] * e.ga[j] - rstd * (v[j] * ax + e.a[j] * vx);
-        gx[j] = rstd * (h - hm - e.xh[j] * hx) - sv * rstd * rstd * e.xh[j];
-        dg[j] = e.g1[j] * t + q[j] * e.xh[j];
-      }
-      if (p.drop.t) drop_apply(p.drop, e.w, gg);
-      if (p.partial) {
-        float* part = p.partial + (long)blockIdx.x * 2 * p.cols + c;
-        add_partial(part, n, row == blockIdx.x, dg);
-        add_partial(part + p.cols, n, row == blockIdx.x, q);
-      }
-      store8((T*)p.ggy + row * p.ld_ggy + c, n, gg);
-      store8((T*)p.out + row * p.ld_out + c, n, gx);
+      for (int i = 0; i < K; ++i) s[i] += t[i];
     }
+    RowSums<256, K>::run(s, sm, turn);
+    if (threadIdx.x == 0)
+#pragma unroll
+      for (int i = 0; i < K; ++i) p.chunk[item * K + i] = s[i];
   }
+}
+
+// 3: both cotangents and the affine sums of a row group.
+template <typename T, int EPI>
+__global__ __launch_bounds__(256) void ln_bwd2_stream(LnArgs p) {
+  if (EPI) drop_state(p.drop);
+  const int c = (int)((blockIdx.x * 256u + threadIdx.x) * 8), cols = (int)p.cols, n = cols - c;
+  if (n <= 0) return;
+  const float inv = 1.f / (float)cols;
+  const bool curved = EPI == 2 && p.act > 1.f;
+  float ga[8], be[8], dg[8], db[8];
+  load_param<T>(p.gamma, p.param_f32, c, n, 1.f, ga);
+  if (EPI == 2) load_param<T>(p.beta, p.param_f32, c, n, 0.f, be);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) dg[j] = db[j] = 0.f;
+  for (long row = blockIdx.y; row < p.rows; row += gridDim.y) {
+    Eight<EPI, true> e;
+    float v[8], gg[8], gx[8];
+    load8((const T*)p.x + row * p.ld_x + c, n, e.xh);
+    load8((const T*)p.gy + row * p.ld_gy + c, n, e.g);
+    load8((const T*)p.ggx + row * p.ld_ggx + c, n, v);
+    const float mean = p.mean[row], rstd = p.rstd[row];
+    const float* rs = p.row + row * ROW_SUMS;
+    const float am = rs[0] * inv, ax = rs[1] * inv, vm = rs[2] * inv, vx = rs[3] * inv;
+    const float sv = rs[4] * inv - vm * am - vx * ax;
+    const float q0 = curved ? rs[5] * inv : 0.f, q1 = curved ? rs[6] * inv : 0.f;
+    const float c0 = rstd * (rstd * am * vx - q0), c1 = -rstd * ax, c2 = -rstd * rstd * vx;
+    const float c3 = -rstd * (q1 + rstd * (sv - vx * ax));
+    e.make(p, row, c, mean, rstd, ga, be);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float t = rstd * (v[j] - vm - e.xh[j] * vx);
+      const float q = EPI == 2 ? e.g[j] * e.d2[j] * ga[j] * t : 0.f, g1 = EPI == 2 ? e.g[j] * e.d1[j] : e.g[j];
+      gg[j] = (EPI == 2 ? e.d1[j] * ga[j] : ga[j]) * t;
+      gx[j] = fmaf(t, c1, fmaf(g1 * ga[j], c2, fmaf(e.xh[j], c3, c0)));
+      dg[j] = fmaf(g1, t, dg[j]);
+      if (EPI == 2) {
+        gx[j] = fmaf(q * ga[j], rstd, gx[j]);
+        dg[j] = fmaf(q, e.xh[j], dg[j]);
+        db[j] += q;
+      }
+    }
+    if (EPI && p.drop.t) drop_apply(p.drop, e.w, gg);
+    store8((T*)p.ggy + row * p.ld_ggy + c, n, gg);
+    store8((T*)p.out + row * p.ld_out + c, n, gx);
+  }
+  if (p.partial) {
+    float* part = p.partial + (long)blockIdx.y * 2 * cols + c;
+    store8(part, n, dg);
+    store8(part + cols, n, db);
+  }
+}
+
+template <typename T, int EPI>
+void launch_split(const LnArgs& a, hipStream_t st) {
+  const long chunks = ln_chunks(a.cols);
+  const unsigned items = ln_items(a.rows, a.cols);
+  ln_bwd2_chunks<T, EPI, false><<<items, 256, 0, st>>>(a, chunks);
+  ln_join<5><<<ln_join_grid(a.rows), 256, 0, st>>>(a.chunk, a.rows, chunks, a.row, 0);
+  if (EPI == 2 && a.act > 1.f) {
+    ln_bwd2_chunks<T, EPI, true><<<items, 256, 0, st>>>(a, chunks);
+    ln_join<2><<<ln_join_grid(a.rows), 256, 0, st>>>(a.chunk, a.rows, chunks, a.row, 5);
+  }
+  ln_bwd2_stream<T, EPI><<<ln_stream_grid(a.rows, a.cols), 256, 0, st>>>(a);
 }
 
 template <typename T>
 void launch(const LnArgs& a, int groups, hipStream_t st) {
   const LnShape s = ln_bwd_shape(a.cols);
   if (s.g == 0) {
-    ln_bwd2_long<T><<<groups, 1024, 0, st>>>(a);
+    if (a.act != 1.f) launch_split<T, 2>(a, st);
+    else if (a.drop.t) launch_split<T, 1>(a, st);
+    else launch_split<T, 0>(a, st);
     return;
   }
 #define SHAPE(G, NV)                                                                                      \
@@ -282,7 +328,7 @@ extern "C" int fcd_layernorm_bwd2(const FcdLayerNormDesc* d, const void* ggx, co
   FCD_TRY(fcd_check_apart(who, out[0], out[1], d->rows, d->cols, es, false));
   FCD_TRY(ln_check_vectors(who, d, gamma, beta, mean, rstd));
   FCD_REQUIRE(d->rows == 0 || (mean && rstd), "%s: mean / rstd are NULL", who);
-  FCD_TRY(ln_check_affine(who, d, 1, dgamma, dbeta, workspace, workspace_bytes, &a));
+  FCD_TRY(ln_check_scratch(who, d, FCD_LN_BWD2, dgamma, dbeta, workspace, workspace_bytes, &a));
   a.x = x, a.gy = gy, a.ggx = ggx, a.gamma = gamma, a.beta = beta, a.out = gx, a.ggy = ggy;
   a.mean = (float*)mean, a.rstd = (float*)rstd;
   const int groups = ln_groups(d->rows, d->cols);

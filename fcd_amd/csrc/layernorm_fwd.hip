@@ -108,63 +108,100 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_fwd_rows(LnArgs p) {
   }
 }
 
-// Rows too long for registers: one workgroup per row, the row read again from cache for every pass.
+// Split rows, 1: mean and sum of squares around it of a chunk.
 template <typename T>
-__global__ __launch_bounds__(1024) void ln_fwd_long(LnArgs p) {
-  constexpr int TH = 1024;
-  __shared__ float sm[2 * TH / 64];
+__global__ __launch_bounds__(256) void ln_fwd_chunks(LnArgs p, long chunks) {
+  __shared__ float sm[2 * 4];
   int turn = 0;
-  drop_state(p.drop);
-  for (long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+  for (long item = blockIdx.x; item < p.rows * chunks; item += gridDim.x) {
+    const long row = item / chunks, c0 = (item - row * chunks) * CHUNK;
     const T* x = (const T*)p.x + row * p.ld_x;
-    float s[1] = {0.f};
-    for (long c = threadIdx.x * 8; c < p.cols; c += TH * 8) {
-      float v[8];
-      load8(x + c, p.cols - c, v);
-      s[0] += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+    const float count = (float)(p.cols - c0 < CHUNK ? p.cols - c0 : CHUNK);
+    float v[4][8], s[1] = {0.f};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const long c = c0 + (threadIdx.x + k * 256) * 8;
+      load8(x + c, p.cols - c, v[k]);
+      s[0] += ((v[k][0] + v[k][1]) + (v[k][2] + v[k][3])) + ((v[k][4] + v[k][5]) + (v[k][6] + v[k][7]));
     }
-    RowSums<TH, 1>::run(s, sm, turn);
-    const float mean = s[0] / (float)p.cols;
+    RowSums<256, 1>::run(s, sm, turn);
+    const float mean = s[0] / count;
     s[0] = 0.f;
-    for (long c = threadIdx.x * 8; c < p.cols; c += TH * 8) {
-      const long n = p.cols - c;
-      float v[8], q = 0.f;
-      load8(x + c, n, v);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const long n = p.cols - c0 - (threadIdx.x + k * 256) * 8;
+      float q = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float d = j < n ? v[j] - mean : 0.f;
+        const float d = j < n ? v[k][j] - mean : 0.f;
         q = fmaf(d, d, q);
       }
       s[0] += q;
     }
-    RowSums<TH, 1>::run(s, sm, turn);
-    const float rstd = 1.f / sqrtf(s[0] / (float)p.cols + p.eps);
-    if (threadIdx.x == 0 && p.mean) {
-      p.mean[row] = mean;
-      p.rstd[row] = rstd;
+    RowSums<256, 1>::run(s, sm, turn);
+    if (threadIdx.x == 0) {
+      p.chunk[item * 2] = mean;
+      p.chunk[item * 2 + 1] = s[0];
     }
-    for (long c = threadIdx.x * 8; c < p.cols; c += TH * 8) {
-      const long n = p.cols - c;
-      float v[8], u[8], ga[8], be[8];
-      load8(x + c, n, v);
-      load_param<T>(p.gamma, p.param_f32, c, n, 1.f, ga);
-      load_param<T>(p.beta, p.param_f32, c, n, 0.f, be);
+  }
+}
+
+// 2: the chunks of a row joined: sum of squares = those around the chunks' means + the means' own spread.
+__global__ __launch_bounds__(256) void ln_fwd_join(LnArgs p, long chunks) {
+  const int lane = threadIdx.x & 63;
+  const float cols = (float)p.cols, last = (float)(p.cols - (chunks - 1) * CHUNK);
+  for (long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6); row < p.rows; row += (long)gridDim.x * 4) {
+    const float* part = p.chunk + row * chunks * 2;
+    float s = 0.f, q = 0.f;
+    for (long i = lane; i < chunks; i += 64) s += part[i * 2] * (i + 1 < chunks ? (float)CHUNK : last);
+    const float mean = lanes_sum<64>(s) / cols;
+    for (long i = lane; i < chunks; i += 64) {
+      const float d = part[i * 2] - mean;
+      q += fmaf(d * d, i + 1 < chunks ? (float)CHUNK : last, part[i * 2 + 1]);
+    }
+    const float rstd = 1.f / sqrtf(lanes_sum<64>(q) / cols + p.eps);
+    if (lane == 0) {
+      p.row[row * 2] = mean;
+      p.row[row * 2 + 1] = rstd;
+      if (p.mean) {
+        p.mean[row] = mean;
+        p.rstd[row] = rstd;
+      }
+    }
+  }
+}
+
+// 3: the result.
+template <typename T>
+__global__ __launch_bounds__(256) void ln_fwd_stream(LnArgs p) {
+  drop_state(p.drop);
+  const long c = ((long)blockIdx.x * 256 + threadIdx.x) * 8, n = p.cols - c;
+  if (n <= 0) return;
+  float ga[8], be[8];
+  load_param<T>(p.gamma, p.param_f32, c, n, 1.f, ga);
+  load_param<T>(p.beta, p.param_f32, c, n, 0.f, be);
+  for (long row = blockIdx.y; row < p.rows; row += gridDim.y) {
+    const float mean = p.row[row * 2], rstd = p.row[row * 2 + 1];
+    float v[8], u[8], r[8];
+    load8((const T*)p.x + row * p.ld_x + c, n, v);
+    if (p.res) load8((const T*)p.res + row * p.ld_res + c, n, r);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) u[j] = fmaf((v[j] - mean) * rstd, ga[j], be[j]);
+    for (int j = 0; j < 8; ++j) u[j] = fmaf((v[j] - mean) * rstd, ga[j], be[j]);
+    if (p.act != 1.f) {
       ln_act8(u, p.act, v, nullptr, nullptr);
-      if (p.drop.t) {
-        uint32_t w[4];
-        drop_draw8(p.drop, (uint64_t)(row * p.cols + c), w);
-        drop_apply(p.drop, w, v);
-      }
-      if (p.res) {
-        float r[8];
-        load8((const T*)p.res + row * p.ld_res + c, n, r);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] += r[j];
-      }
-      store8((T*)p.out + row * p.ld_out + c, n, v);
+      for (int j = 0; j < 8; ++j) u[j] = v[j];
     }
+    if (p.drop.t) {
+      uint32_t w[4];
+      drop_draw8(p.drop, (uint64_t)(row * p.cols + c), w);
+      drop_apply(p.drop, w, u);
+    }
+    if (p.res) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) u[j] += r[j];
+    }
+    store8((T*)p.out + row * p.ld_out + c, n, u);
   }
 }
 
@@ -183,13 +220,17 @@ void launch(const LnArgs& a, hipStream_t st) {
   }
   LN_FWD_SHAPES(SHAPE)
 #undef SHAPE
-  ln_fwd_long<T><<<(unsigned)(a.rows < 65536 ? a.rows : 65536), 1024, 0, st>>>(a);
+  const long chunks = ln_chunks(a.cols);
+  ln_fwd_chunks<T><<<ln_items(a.rows, a.cols), 256, 0, st>>>(a, chunks);
+  ln_fwd_join<<<ln_join_grid(a.rows), 256, 0, st>>>(a, chunks);
+  ln_fwd_stream<T><<<ln_stream_grid(a.rows, a.cols), 256, 0, st>>>(a);
 }
 
 }  // namespace
 
 extern "C" int fcd_layernorm_fwd(const FcdLayerNormDesc* d, const void* x, const void* gamma, const void* beta,
-                                 const void* residual, void* y, float* mean, float* rstd, void* stream) {
+                                 const void* residual, void* y, float* mean, float* rstd, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
   const char* who = "fcd_layernorm_fwd";
   LnArgs a;
   FCD_TRY(ln_check(who, d, &a));
@@ -202,6 +243,7 @@ extern "C" int fcd_layernorm_fwd(const FcdLayerNormDesc* d, const void* x, const
   FCD_TRY(fcd_check_apart(who, vy, vr, d->rows, d->cols, es, true));
   FCD_TRY(ln_check_vectors(who, d, gamma, beta, mean, rstd));
   FCD_REQUIRE(!mean == !rstd, "%s: mean and rstd go together", who);
+  FCD_TRY(ln_check_scratch(who, d, FCD_LN_FWD, nullptr, nullptr, workspace, workspace_bytes, &a));
   if (d->rows == 0) return FCD_OK;
   a.x = x, a.gamma = gamma, a.beta = beta, a.res = residual, a.out = y, a.mean = mean, a.rstd = rstd;
   hipStream_t st = fcd_stream(stream);

@@ -885,25 +885,29 @@ def _ln_stat(t, name, d, x):
     return t.data_ptr()
 
 
-def _ln_affine(gamma, beta, want_affine, dgamma, dbeta, accumulate, d, x, second):
-    """Gradient tensors of the affine parameters (given, fresh, or None) and the scratch their row sums need."""
+def _ln_affine(gamma, beta, want_affine, dgamma, dbeta, accumulate, d, x):
+    """Gradient tensors of the affine parameters: given, fresh, or None."""
     if not want_affine:
-        return None, None, None, 0
+        return None, None
     if dgamma is None and dbeta is None:
         if accumulate:
             raise RuntimeError("fcd_amd: accumulate needs dgamma / dbeta")
-        dgamma = None if gamma is None else torch.empty_like(gamma)
-        dbeta = None if beta is None else torch.empty_like(beta)
-    else:
-        for t, name in ((dgamma, "dgamma"), (dbeta, "dbeta")):
-            if t is not None and (_DT.get(t.dtype) != d.param_dtype or t.get_device() != x.get_device()
-                                  or t.numel() != d.cols or not t.is_contiguous()):
-                raise RuntimeError(f"fcd_amd: {name} must be a contiguous vector of {d.cols} elements of the parameters' type")
-    if dgamma is None and dbeta is None:
-        return None, None, None, 0
-    n = L.load().fcd_layernorm_workspace_bytes(C.byref(d), second)
+        return None if gamma is None else torch.empty_like(gamma), None if beta is None else torch.empty_like(beta)
+    for t, name in ((dgamma, "dgamma"), (dbeta, "dbeta")):
+        if t is not None and (_DT.get(t.dtype) != d.param_dtype or t.get_device() != x.get_device() or t.numel() != d.cols
+                              or not t.is_contiguous()):
+            raise RuntimeError(f"fcd_amd: {name} must be a contiguous vector of {d.cols} elements of the parameters' type")
+    return dgamma, dbeta
+
+
+LN_FWD, LN_BWD, LN_BWD2 = 0, 1, 2      # FCD_LN_*
+LN_WHOLE = 8192                        # FCD_LN_WHOLE
+
+
+def _ln_scratch(d, which, affine, x):
+    n = L.load().fcd_layernorm_workspace_bytes(C.byref(d), which, affine)
     # a buffer of this call's own: inside a captured graph it belongs to that graph's memory
-    return dgamma, dbeta, x.new_empty(n, dtype=torch.uint8) if n else None, n
+    return (x.new_empty(n, dtype=torch.uint8) if n else None), n
 
 
 def layernorm_fwd(x: torch.Tensor, gamma=None, beta=None, eps: float = LN_EPS, act_slope: float = 1.0, p: float = 0.0,
@@ -922,8 +926,9 @@ def layernorm_fwd(x: torch.Tensor, gamma=None, beta=None, eps: float = LN_EPS, a
         d.ld_out = _row_operand(out, "out", x)
     mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
     rstd = torch.empty_like(mean)
+    ws, wn = (None, 0) if d.cols <= LN_WHOLE else _ln_scratch(d, LN_FWD, 0, x)
     check(L.load().fcd_layernorm_fwd(C.byref(d), x.data_ptr(), ptr(gamma), ptr(beta), ptr(residual), out.data_ptr(),
-                                     mean.data_ptr(), rstd.data_ptr(), stream()), "layernorm_fwd")
+                                     mean.data_ptr(), rstd.data_ptr(), ptr(ws), wn, stream()), "layernorm_fwd")
     return out, mean, rstd
 
 
@@ -940,7 +945,8 @@ def layernorm_bwd(gy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: t
         d.ld_out = d.cols
     else:
         d.ld_out = _row_operand(out, "out", x)
-    dgamma, dbeta, ws, wn = _ln_affine(gamma, beta, want_affine, dgamma, dbeta, accumulate, d, x, 0)
+    dgamma, dbeta = _ln_affine(gamma, beta, want_affine, dgamma, dbeta, accumulate, d, x)
+    ws, wn = _ln_scratch(d, LN_BWD, dgamma is not None or dbeta is not None, x)
     check(L.load().fcd_layernorm_bwd(C.byref(d), gy.data_ptr(), x.data_ptr(), _ln_stat(mean, "mean", d, x),
                                      _ln_stat(rstd, "rstd", d, x), ptr(gamma), ptr(beta), out.data_ptr(), ptr(dgamma),
                                      ptr(dbeta), int(accumulate), ptr(ws), wn, stream()), "layernorm_bwd")
@@ -962,7 +968,8 @@ def layernorm_bwd2(ggx: torch.Tensor, gy: torch.Tensor, x: torch.Tensor, mean: t
     else:
         ggy, gx = outs
         d.ld_ggy, d.ld_out = _row_operand(ggy, "ggy", x), _row_operand(gx, "gx", x)
-    dgamma, dbeta, ws, wn = _ln_affine(gamma, beta, want_affine, dgamma, dbeta, accumulate, d, x, 1)
+    dgamma, dbeta = _ln_affine(gamma, beta, want_affine, dgamma, dbeta, accumulate, d, x)
+    ws, wn = _ln_scratch(d, LN_BWD2, dgamma is not None or dbeta is not None, x)
     check(L.load().fcd_layernorm_bwd2(C.byref(d), ggx.data_ptr(), gy.data_ptr(), x.data_ptr(), _ln_stat(mean, "mean", d, x),
                                       _ln_stat(rstd, "rstd", d, x), ptr(gamma), ptr(beta), ggy.data_ptr(), gx.data_ptr(),
                                       ptr(dgamma), ptr(dbeta), int(accumulate), ptr(ws), wn, stream()), "layernorm_bwd2")

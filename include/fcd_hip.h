@@ -515,13 +515,17 @@ typedef struct FcdLayerNormDesc {
 } FcdLayerNormDesc;
 
 int fcd_layernorm_desc_bytes(void);
+/* Scratch of a pass (FCD_LN_*); affine: with dgamma / dbeta.  0: none is needed, NULL will do. */
+#define FCD_LN_FWD 0
+#define FCD_LN_BWD 1
+#define FCD_LN_BWD2 2
+#define FCD_LN_WHOLE 8192 /* rows of up to this many columns are never split: their forward pass needs no scratch */
+size_t fcd_layernorm_workspace_bytes(const FcdLayerNormDesc* d, int pass, int affine);
 /* y = drop(act((x - mean) * rstd * gamma + beta)) (+ residual).  gamma NULL: 1; beta NULL: 0; mean and rstd (outputs) may
  * both be NULL. */
 int fcd_layernorm_fwd(const FcdLayerNormDesc* d, const void* x, const void* gamma, const void* beta,
-                      const void* residual, void* y, float* mean, float* rstd, void* stream);
-/* Scratch of fcd_layernorm_bwd (second 0) / _bwd2 (second 1) when they compute dgamma / dbeta (none without them); 0: none
- * is needed, NULL will do. */
-size_t fcd_layernorm_workspace_bytes(const FcdLayerNormDesc* d, int second);
+                      const void* residual, void* y, float* mean, float* rstd, void* workspace, size_t workspace_bytes,
+                      void* stream);
 /* With u = xhat * gamma + beta, g1 = drop(gy) * act'(u), a = g1 * gamma:
  *   dx = rstd * (a - mean(a) - xhat * mean(a * xhat)),  dgamma (+)= sum_rows g1 * xhat,  dbeta (+)= sum_rows g1.
  * (residual's gradient is gy itself.)  dgamma / dbeta NULL: not computed.  Row sums in a fixed order, no atomics. */

@@ -80,7 +80,7 @@ def test_descriptors_refused(over, text):
     from fcd_amd import _lib
     lib, d = _lib.load(), C.byref(desc(**over))
     f = lambda i: P * 64 * i
-    refused(lib.fcd_layernorm_fwd(d, f(1), None, None, None, f(2), f(3), f(4), None), text)
+    refused(lib.fcd_layernorm_fwd(d, f(1), None, None, None, f(2), f(3), f(4), None, 0, None), text)
     refused(lib.fcd_layernorm_bwd(d, f(1), f(2), f(3), f(4), None, None, f(5), None, None, 0, None, 0, None), text)
     refused(lib.fcd_layernorm_bwd2(d, f(1), f(2), f(3), f(4), f(5), None, None, f(6), f(7), None, None, 0, None, 0, None), text)
 
@@ -88,12 +88,13 @@ def test_descriptors_refused(over, text):
 @pytest.mark.parametrize("eps", [-1e-5, float("nan"), float("inf")])
 def test_eps_refused(eps):
     from fcd_amd import _lib
-    refused(_lib.load().fcd_layernorm_fwd(C.byref(desc(eps=eps)), P, None, None, None, 2 * P, None, None, None), "eps")
+    refused(_lib.load().fcd_layernorm_fwd(C.byref(desc(eps=eps)), P, None, None, None, 2 * P, None, None, None, 0, None), "eps")
 
 
 def test_forward_operands_refused():
     from fcd_amd import _lib
-    fwd = _lib.load().fcd_layernorm_fwd
+    lib = _lib.load()
+    fwd = lambda *a: lib.fcd_layernorm_fwd(*a[:-1], None, 0, a[-1])
     d = C.byref(desc())
     refused(fwd(None, P, None, None, None, 2 * P, None, None, None), "NULL descriptor")
     refused(fwd(d, None, None, None, None, P, None, None, None), "x is NULL")
@@ -115,7 +116,7 @@ def test_backward_operands_refused():
     from fcd_amd import _lib
     lib = _lib.load()
     d = desc(rows=400)
-    need = lib.fcd_layernorm_workspace_bytes(C.byref(d), 0)
+    need = lib.fcd_layernorm_workspace_bytes(C.byref(d), 1, 1)
     assert need >= 2 * 16 * 4
     f = lambda i: P * i
     call = lambda **k: lib.fcd_layernorm_bwd(C.byref(d), *[{**dict(gy=f(1), x=f(2), mean=f(3), rstd=f(4), ga=None, be=None, dx=f(5),
@@ -133,10 +134,22 @@ def test_backward_operands_refused():
     refused(d2(f(1), f(2), f(3), f(4), f(5), None, None, f(6), f(1) + 8, None, None, 0, None, 0, None), "overlaps ggx")
     refused(d2(None, f(2), f(3), f(4), f(5), None, None, f(6), f(7), None, None, 0, None, 0, None), "ggx is NULL")
     refused(d2(f(1), f(2), f(3), f(4), f(5), None, None, f(6), f(7), f(8), None, 0, f(9), 8, None), "workspace", -2)
-    for second in (0, 1):
-        assert lib.fcd_layernorm_workspace_bytes(None, second) == 0
-        assert lib.fcd_layernorm_workspace_bytes(C.byref(desc(rows=0)), second) == 0
-    assert lib.fcd_layernorm_workspace_bytes(C.byref(desc(rows=4)), 1) >= 2 * 16 * 4
+    for which in (0, 1, 2):
+        assert lib.fcd_layernorm_workspace_bytes(None, which, 1) == 0
+        assert lib.fcd_layernorm_workspace_bytes(C.byref(desc(rows=0)), which, 1) == 0
+    small = C.byref(desc(rows=4))
+    assert lib.fcd_layernorm_workspace_bytes(small, 0, 1) == 0            # the forward pass and few rows need none
+    assert lib.fcd_layernorm_workspace_bytes(small, 1, 1) == 0
+    assert lib.fcd_layernorm_workspace_bytes(small, 2, 1) >= 2 * 16 * 4
+    assert lib.fcd_layernorm_workspace_bytes(small, 2, 0) == 0
+    # split rows need some in every pass, with or without affine gradients
+    n = 40000
+    wide = desc(rows=4, cols=n, ld_x=n, ld_gy=n, ld_ggx=n, ld_out=n, ld_ggy=n)
+    for which in (0, 1, 2):
+        assert lib.fcd_layernorm_workspace_bytes(C.byref(wide), which, 0) > 0
+    refused(lib.fcd_layernorm_fwd(C.byref(wide), f(1), None, None, None, f(2), None, None, None, 0, None), "workspace", -2)
+    refused(lib.fcd_layernorm_bwd(C.byref(wide), f(1), f(2), f(3), f(4), None, None, f(5), None, None, 0, None, 0, None),
+            "workspace", -2)
 
 
 def test_dropout_refused():

@@ -445,6 +445,9 @@ def test_more_than_32_bits_of_elements(dev):
         R.check(z[i], R.V(xd * m, 2 * R.U * (xd * m).abs()), BF16, "dropout")
 
 
-def test_very_long_rows(dev):
-    run_all(dev, 2, 300007, F32, 2.0, 0.1)
-    run_all(dev, 3, 131080, BF16, 1.0, 0.0)
+@pytest.mark.parametrize("rows,cols", [(1, 65536), (2, 300007), (3, 131080), (5, 8193), (300, 16385), (700, 8200)])
+def test_split_rows(dev, rows, cols):
+    """Rows longer than a workgroup's registers, with one chunk of the row nearly empty and with ragged ends."""
+    run_all(dev, rows, cols, F32, 2.0, 0.1)
+    run_all(dev, rows, cols, BF16, 1.0, 0.0, pad=3, residual=True)
+    run_all(dev, rows, cols, F16, 0.01, 0.4, seed=2)
