@@ -4,30 +4,54 @@
 
 namespace {
 
-// 8 elements a thread and turn: x and the residual in, y out, one generator block between.  A workgroup stays in one row
-// (blockIdx.y and further rows below it); a tensor without gaps is one long row.
-template <typename T>
+// 8 elements a thread and turn: x and the residual in, y out, one generator block between.  The units of a row start at the
+// generator's blocks, not at the row's first element (memory takes any alignment; half a block would cost a whole one), so
+// that a row's first unit may begin late and its last end early.  256 threads a row (WIDE), or 2^lt of them and several rows
+// a workgroup; a tensor without gaps is one long row.
+template <typename T, bool WIDE>
 __global__ __launch_bounds__(256) void dropout_kernel(const T* x, const T* res, T* y, long rows, long cols, long ld_x,
-                                                      long ld_res, long ld_y, Drop d) {
+                                                      long ld_res, long ld_y, int lt, Drop d) {
   drop_state(d);
-  for (long row = blockIdx.y; row < rows; row += gridDim.y) {
+  if (WIDE) lt = 8;
+  const int per_row = 1 << lt, rpb = 256 >> lt;
+  for (long row = (long)blockIdx.y * rpb + (WIDE ? 0 : threadIdx.x >> lt); row < rows; row += (long)gridDim.y * rpb) {
     const T *xr = x + row * ld_x, *rr = res + row * ld_res;
     T* yr = y + row * ld_y;
-    for (long c = ((long)blockIdx.x * 256 + threadIdx.x) * 8; c < cols; c += (long)gridDim.x * 256 * 8) {
-      const long n = cols - c;
-      float v[8], r[8];
-      load8(xr + c, n, v);
-      if (res) load8(rr + c, n, r);
-      if (d.t) {
-        uint32_t w[4];
-        drop_draw8(d, (uint64_t)(row * cols + c), w);
-        drop_apply(d, w, v);
-      }
-      if (res) {
+    const int phase = (int)((row * cols) & 7);
+    const uint64_t first = (uint64_t)(row * cols - phase);
+    for (long u = ((long)blockIdx.x * per_row + (threadIdx.x & (per_row - 1))) * 8; u < cols + phase;
+         u += (long)gridDim.x * per_row * 8) {
+      const long c = u - phase;
+      uint32_t w[4];
+      if (c >= 0 && c + 8 <= cols) {
+        typedef typename Oct<T>::type O;
+        const O ox = *reinterpret_cast<const O*>(xr + c);
+        O orr = {};
+        if (res) orr = *reinterpret_cast<const O*>(rr + c);
+        float v[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] += r[j];
+        for (int j = 0; j < 8; ++j) v[j] = (float)ox[j];
+        if (d.t) {
+          drop_block(d, d.offset + ((first + u) >> 3), w);
+          drop_apply(d, w, v);
+        }
+        O o;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] = (T)(res ? v[j] + (float)orr[j] : v[j]);
+        *reinterpret_cast<O*>(yr + c) = o;
+      } else {
+        if (d.t) drop_block(d, d.offset + ((first + u) >> 3), w);
+        for (int j = 0; j < 8; ++j) {
+          if (c + j < 0 || c + j >= cols) continue;
+          float v = (float)xr[c + j];
+          if (d.t) {
+            const uint32_t h = j < 2 ? w[0] : j < 4 ? w[1] : j < 6 ? w[2] : w[3];
+            v = (j & 1 ? h : h << 16) > d.below ? v * d.scale : 0.f;
+          }
+          if (res) v += (float)rr[c + j];
+          yr[c + j] = (T)v;
+        }
       }
-      store8(yr + c, n, v);
     }
   }
 }
@@ -62,14 +86,23 @@ extern "C" int fcd_dropout(const void* x, const void* residual, void* y, int64_t
     cols *= rows;
     rows = 1;
   }
-  const int64_t bx = (cols + 2047) / 2048;
-  const dim3 grid((unsigned)(bx < (1 << 20) ? bx : (1 << 20)), (unsigned)(rows < 32768 ? rows : 32768));
+  int lt = 0;
+  while (lt < 8 && ((int64_t)8 << lt) < cols + 7) ++lt;
+  const int64_t bx = lt < 8 ? 1 : (cols + 7 + 2047) / 2048, by = (rows + (256 >> lt) - 1) / (256 >> lt);
+  const dim3 grid((unsigned)(bx < (1 << 20) ? bx : (1 << 20)), (unsigned)(by < 32768 ? by : 32768));
   hipStream_t st = fcd_stream(stream);
-#define LAUNCH(T)                                                                                                     \
-  dropout_kernel<T><<<grid, 256, 0, st>>>((const T*)x, (const T*)residual, (T*)y, rows, cols, ld_x, ld_res, ld_y, d)
-  if (dtype == FCD_DT_F32) LAUNCH(float);
-  else if (dtype == FCD_DT_BF16) LAUNCH(bf16_t);
-  else LAUNCH(f16_t);
+#define LAUNCH(T)                                                                                                            \
+  if (lt == 8)                                                                                                                \
+    dropout_kernel<T, true><<<grid, 256, 0, st>>>((const T*)x, (const T*)residual, (T*)y, rows, cols, ld_x, ld_res, ld_y, lt, d); \
+  else                                                                                                                        \
+    dropout_kernel<T, false><<<grid, 256, 0, st>>>((const T*)x, (const T*)residual, (T*)y, rows, cols, ld_x, ld_res, ld_y, lt, d)
+  if (dtype == FCD_DT_F32) {
+    LAUNCH(float);
+  } else if (dtype == FCD_DT_BF16) {
+    LAUNCH(bf16_t);
+  } else {
+    LAUNCH(f16_t);
+  }
 #undef LAUNCH
   return fcd_check_launch(who);
 }

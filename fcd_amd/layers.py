@@ -32,10 +32,8 @@ def _even(t: torch.Tensor) -> torch.Tensor:
 class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, eps, act, p, rng):
-        x = _even(x)
-        residual = None if residual is None else _even(residual)
-        y, mean, rstd = ops.layernorm_fwd(x, weight, bias, eps, act, p, rng, residual)
-        ctx.save_for_backward(x, weight, bias, mean, rstd)
+        y, mean, rstd = ops.layernorm_fwd(_even(x), weight, bias, eps, act, p, rng, None if residual is None else _even(residual))
+        ctx.save_for_backward(x, weight, bias, mean, rstd)      # (x itself, not a copy: the second backward leads to it)
         ctx.cfg = act, p, rng
         ctx.set_materialize_grads(False)
         return y
@@ -58,7 +56,7 @@ class _LayerNormBwdFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, gy, x, weight, bias, mean, rstd, cfg, want_affine):
-        gy = _even(gy)
+        gy, x = _even(gy), _even(x)
         act, p, rng = cfg
         ctx.save_for_backward(gy, x, weight, bias, mean, rstd)
         ctx.cfg = cfg

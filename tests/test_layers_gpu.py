@@ -139,6 +139,26 @@ def test_layer_norm_module(dev):
         LayerNorm(8, dropout=1.5)
 
 
+@pytest.mark.parametrize("layout", ["transposed", "every second column", "expanded"])
+def test_inputs_without_even_rows(dev, layout):
+    """Layouts the kernels do not take are copied; first and second gradients still reach the tensor that was given."""
+    from fcd_amd import layers
+    g = torch.Generator().manual_seed(2)
+    base = {"transposed": torch.randn(24, 10, generator=g), "every second column": torch.randn(10, 48, generator=g),
+            "expanded": torch.randn(10, 1, generator=g)}[layout].to(dev).requires_grad_(True)
+    view = {"transposed": lambda t: t.t(), "every second column": lambda t: t[:, ::2], "expanded": lambda t: t.expand(10, 24)}[layout]
+    w = torch.linspace(0.5, 1.5, 24, device=dev)
+    gy, v = torch.randn(10, 24, generator=g).to(dev), torch.randn(base.shape, generator=g).to(dev)
+    res = []
+    for x in (view(base), view(base).contiguous()):
+        y = layers.layer_norm(x, w, activation="silu", residual=x)
+        dx, = torch.autograd.grad(y, base, gy, create_graph=True)
+        res.append((y, dx, torch.autograd.grad(dx, base, v)[0]))
+    assert all(torch.equal(a, b) for a, b in zip(*res))
+    y = layers.dropout(view(base), 0.5, (1, 2))
+    assert torch.equal(y, layers.dropout(view(base).contiguous(), 0.5, (1, 2)))
+
+
 def test_parameter_gradients_are_not_differentiable(dev):
     from fcd_amd import layers
     x = torch.randn(4, 16, device=dev, requires_grad=True)
