@@ -216,6 +216,19 @@ struct RowSums {
   }
 };
 
+// A wave without elements (a row of 1536 has 192 units for 256 threads): its part in a row's sums is their barriers and a
+// zero.  It leaves the rest of the row loop out, to the gain of the other waves on its SIMD.
+template <int G>
+__device__ __forceinline__ bool idle_wave(int cols) {
+  return G > 64 && __builtin_amdgcn_readfirstlane(threadIdx.x & ~63u) * 8 >= cols;
+}
+
+template <int G, int K>
+__device__ __forceinline__ void idle_sums(float* sm, int& turn) {
+  float s[K] = {};
+  RowSums<G, K>::run(s, sm, turn);
+}
+
 // ---------------------------------------------------------------- activations ----------
 // The smooth ones from one hardware exponential and one hardware reciprocal (a step of fp32 each).  exp(u) as 2^(u log2 e)
 // loses |u| / 2 steps relative; what it is used in changes by at most |u| s (1 - s) < 0.23 times that.

@@ -43,7 +43,10 @@ __device__ __forceinline__ void bwd_rows(LnArgs p, unsigned blocks) {
   // G < 64: every thread of a wave makes the same number of turns, for the sums need whole groups; G >= 64: whole waves do
   long row = first_row<G, TH>();
   const long step = (long)blocks * RPB;
-  const long turns = (p.rows - (G >= 64 ? row : (long)blockIdx.x * RPB) + step - 1) / step;
+  long turns = (p.rows - (G >= 64 ? row : (long)blockIdx.x * RPB) + step - 1) / step;
+  if (idle_wave<G>(cols)) {
+    for (; turns > 0; --turns) idle_sums<G, 2>(sm, turn);
+  }
   if (turns > 0) fetch(row);
 #pragma unroll
   for (int k = 0; k < NV; ++k) {

@@ -45,7 +45,13 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd2_rows(LnArgs p) {
   // G < 64: every thread of a wave makes the same number of turns, for the sums need whole groups; G >= 64: whole waves do
   long row = first_row<G, TH>();
   const long step = (long)gridDim.x * RPB;
-  const long turns = (p.rows - (G >= 64 ? row : (long)blockIdx.x * RPB) + step - 1) / step;
+  long turns = (p.rows - (G >= 64 ? row : (long)blockIdx.x * RPB) + step - 1) / step;
+  if (idle_wave<G>(cols)) {
+    for (; turns > 0; --turns) {
+      idle_sums<G, 5>(sm, turn);
+      if (curved) idle_sums<G, 2>(sm2, turn2);
+    }
+  }
   // a workgroup of 1024 has 128 registers a thread: behind an activation they do not hold the next row as well
   constexpr bool AHEAD = !(G == 1024 && EPI == 2);
   if (AHEAD && turns > 0) fetch(row);

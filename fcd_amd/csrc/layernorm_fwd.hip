@@ -34,6 +34,13 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_fwd_rows(LnArgs p) {
   long row = first_row<G, TH>();
   const long step = (long)gridDim.x * RPB;
   const long turns = (p.rows - (G >= 64 ? row : (long)blockIdx.x * RPB) + step - 1) / step;
+  if (idle_wave<G>(cols)) {
+    for (long it = 0; it < turns; ++it) {
+      idle_sums<G, 1>(sm, turn);
+      idle_sums<G, 1>(sm, turn);
+    }
+    return;
+  }
   if (turns > 0) fetch(p.x, p.ld_x, row, nx);
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
@@ -80,6 +87,7 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_fwd_rows(LnArgs p) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int c = (lane + k * G) * 8, n = here ? cols - c : 0;
+      if (k > 0 && G >= 64 && (__builtin_amdgcn_readfirstlane(lane & ~63) + k * G) * 8 >= cols) break;   // none in this wave
       float u[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) u[j] = fmaf(v[k][j] * rstd, ga[k][j], be[k][j]);
