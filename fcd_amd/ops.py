@@ -854,28 +854,27 @@ def dropout(x: torch.Tensor, p: float, rng, residual: Optional[torch.Tensor] = N
     return out
 
 
-def _ln_param(t, name, cols, x):
-    if (t.dtype != torch.float32 and t.dtype != x.dtype) or t.get_device() != x.get_device() or t.numel() != cols \
-            or not t.is_contiguous():
-        raise RuntimeError(f"fcd_amd: {name} must be a contiguous float32 or {x.dtype} vector of {cols} elements on {x.device}")
-    return _DT[t.dtype]
-
-
 def _ln_desc(x, gamma, beta, eps, act_slope, p, rng):
     d = L.LayerNormDesc()
-    d.dtype = _here(x, "x")
+    dtype, dev = x.dtype, x.get_device()
+    d.dtype = dt = _here(x, "x")
     d.rows, cols, d.ld_x = _rows(x, "x")
     d.cols = cols
-    if gamma is not None:
-        d.param_dtype = _ln_param(gamma, "gamma", cols, x)
-    if beta is not None:
-        dt = _ln_param(beta, "beta", cols, x)
-        if gamma is not None and dt != d.param_dtype:
+    pdt = None
+    for t, name in ((gamma, "gamma"), (beta, "beta")):
+        if t is None:
+            continue
+        tdt = t.dtype
+        if (tdt is not torch.float32 and tdt is not dtype) or t.get_device() != dev or t.numel() != cols or not t.is_contiguous():
+            raise RuntimeError(f"fcd_amd: {name} must be a contiguous float32 or {dtype} vector of {cols} elements on {x.device}")
+        if pdt is not None and tdt is not pdt:
             raise RuntimeError("fcd_amd: gamma and beta must have one type")
+        pdt = tdt
+    if pdt is dtype:
         d.param_dtype = dt
     d.eps, d.act, d.drop_p = eps, act_slope, p
     if p != 0.0:
-        d.seed, d.offset, d.rng = _rng_words(p, rng, x.get_device())
+        d.seed, d.offset, d.rng = _rng_words(p, rng, dev)
     return d
 
 
@@ -924,7 +923,9 @@ def layernorm_fwd(x: torch.Tensor, gamma=None, beta=None, eps: float = LN_EPS, a
         d.ld_out = d.cols
     else:
         d.ld_out = _row_operand(out, "out", x)
-    mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    mean = torch.empty(d.rows, dtype=torch.float32, device=x.device)
+    if x.dim() != 2:
+        mean = mean.view(x.shape[:-1])
     rstd = torch.empty_like(mean)
     ws, wn = (None, 0) if d.cols <= LN_WHOLE else _ln_scratch(d, LN_FWD, 0, x)
     check(L.load().fcd_layernorm_fwd(C.byref(d), x.data_ptr(), ptr(gamma), ptr(beta), ptr(residual), out.data_ptr(),
