@@ -13,7 +13,7 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_fwd_rows(LnArgs p) {
   int turn = 0;
   if (EPI) drop_state(p.drop);
   const int lane = threadIdx.x % G, cols = (int)p.cols;
-  const float fcols = (float)cols;
+  const float fcols = (float)cols, inv = 1.f / fcols;
   float ga[NV][8], be[NV][8];
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
@@ -62,28 +62,32 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_fwd_rows(LnArgs p) {
     for (int k = 0; k < NV; ++k)
       s[0] += ((v[k][0] + v[k][1]) + (v[k][2] + v[k][3])) + ((v[k][4] + v[k][5]) + (v[k][6] + v[k][7]));
     RowSums<G, 1>::run(s, sm, turn);
-    const float mean = s[0] / fcols;
+    // the quotient, corrected once by its remainder: exact where it is a number (rows without spread), and a tenth of a
+    // division's instructions
+    float mean = s[0] * inv;
+    const float fine = fmaf(fmaf(-mean, fcols, s[0]), inv, mean);
+    mean = fine == fine ? fine : mean;                       // (an infinite sum has no remainder)
     s[0] = 0.f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int n = cols - (lane + k * G) * 8;
       float q = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[k][j] = j < n ? v[k][j] - mean : 0.f;
-        q = fmaf(v[k][j], v[k][j], q);
+      for (int j = 0; j < 8; ++j) v[k][j] -= mean;
+      if (n < 8) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[k][j] = j < n ? v[k][j] : 0.f;
       }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) q = fmaf(v[k][j], v[k][j], q);
       s[0] += q;
     }
     RowSums<G, 1>::run(s, sm, turn);
-    const float rstd = 1.f / sqrtf(s[0] / fcols + p.eps);
+    const float rstd = __builtin_amdgcn_rsqf(fmaf(s[0], inv, p.eps));
     if (lane == 0 && here && p.mean) {
       p.mean[row] = mean;
       p.rstd[row] = rstd;
     }
-    T* out = (T*)p.out + row * p.ld_out;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) arrive<T>(nx[k]);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int c = (lane + k * G) * 8, n = here ? cols - c : 0;
@@ -111,7 +115,16 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_fwd_rows(LnArgs p) {
           for (int j = 0; j < 8; ++j) u[j] += r[j];
         }
       }
-      store8(out + c, n, u);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[k][j] = u[j];
+    }
+    T* out = (T*)p.out + row * p.ld_out;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) arrive<T>(nx[k]);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (lane + k * G) * 8;
+      store8(out + c, here ? cols - c : 0, v[k]);
     }
   }
 }

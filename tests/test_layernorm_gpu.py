@@ -225,6 +225,7 @@ def test_non_finite_rows_stay_alone(dev, cols):
     rest = [i for i in range(16) if i not in (3, 7)]
     assert torch.equal(y1[rest], y[rest]) and torch.equal(r1[rest], rstd[rest])
     assert bool(torch.isnan(y1[3]).all()) and bool(torch.isnan(y1[7]).any())
+    assert bool(torch.isnan(m1[3])) and float(m1[7]) == float("inf")
     dx, _, _ = ops.layernorm_bwd(t["gy"], t["x"], mean, rstd, t["gamma"], t["beta"])
     dx1, _, _ = ops.layernorm_bwd(t["gy"], x, m1, r1, t["gamma"], t["beta"])
     assert torch.equal(dx1[rest], dx[rest]) and bool(torch.isnan(dx1[3]).all())
