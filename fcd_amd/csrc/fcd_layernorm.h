@@ -23,7 +23,7 @@ int ln_check_scratch(const char* who, const FcdLayerNormDesc* d, int pass, const
 int ln_finish(const char* who, const FcdLayerNormDesc* d, const LnArgs& a, int groups, void* dgamma, void* dbeta, int accumulate,
               hipStream_t st);
 int ln_groups(int64_t rows, int64_t cols);   // workgroups (row groups of split rows) of the backward passes
-bool ln_few_rows(int64_t rows, int64_t cols);   // the first backward pass sums its columns beside the rows, in one launch
+bool ln_few_rows(int64_t rows, int64_t cols);   // the first backward pass sums its columns apart from the rows (ln_bwd_few)
 
 // Where a row lives: G threads with NV units of 8 elements each.  G <= 64: the row's sums stay inside a wave, and a workgroup
 // of 256 works on 256 / G rows with no barrier; G > 64: one workgroup per row, one barrier per sum.  The forward pass keeps

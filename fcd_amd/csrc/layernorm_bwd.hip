@@ -144,7 +144,8 @@ __device__ __forceinline__ void put_affine(void* out, int f32, int accumulate, i
 
 // Few rows: the first `blocks` workgroups write dx; the others sum 64 columns each over all rows, which needs nothing from the
 // first ones (the row sums do not enter the affine gradients).  x and gy are read twice, from cache; in exchange there is
-// no scratch and no second launch.
+// no scratch and no second launch: 64 x 2048 fp32 8.4 -> 4.8 us, 128 x 8192 bf16 12.8 -> 5.7.  Up to four turns of a column
+// workgroup: 512 x 2048 (sixteen) takes 10.4 us here and 12.4 in two launches, 256 x 1024 with an activation 12.8 and 8.9.
 template <typename T, int G, int EPI>
 __global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd_few(LnArgs p, Affine f, unsigned blocks) {
   constexpr int TH = G > 64 ? G : 256;
@@ -362,12 +363,16 @@ extern "C" int fcd_layernorm_bwd(const FcdLayerNormDesc* d, const void* gy, cons
   a.x = x, a.gy = gy, a.gamma = gamma, a.beta = beta, a.out = dx, a.mean = (float*)mean, a.rstd = (float*)rstd;
   const int groups = ln_groups(d->rows, d->cols);
   hipStream_t st = fcd_stream(stream);
-  if ((dgamma || dbeta) && ln_few_rows(d->rows, d->cols)) {
+  const bool few = (dgamma || dbeta) && ln_few_rows(d->rows, d->cols);
+  const bool in_place = dx == gy || dx == x;   // dx would overwrite what the column workgroups read: those go first
+  if (few) {
     const Affine f{dgamma, dbeta, accumulate};
-    if (d->dtype == FCD_DT_F32) launch_few<float>(a, f, groups, st);
-    else if (d->dtype == FCD_DT_BF16) launch_few<bf16_t>(a, f, groups, st);
-    else launch_few<f16_t>(a, f, groups, st);
-    return fcd_check_launch(who);
+    const int beside = in_place ? 0 : groups;
+    if (d->dtype == FCD_DT_F32) launch_few<float>(a, f, beside, st);
+    else if (d->dtype == FCD_DT_BF16) launch_few<bf16_t>(a, f, beside, st);
+    else launch_few<f16_t>(a, f, beside, st);
+    FCD_TRY(fcd_check_launch(who));
+    if (!in_place) return FCD_OK;
   }
   if (d->rows) {
     if (d->dtype == FCD_DT_F32) launch<float>(a, groups, st);
@@ -375,6 +380,6 @@ extern "C" int fcd_layernorm_bwd(const FcdLayerNormDesc* d, const void* gy, cons
     else launch<f16_t>(a, groups, st);
     FCD_TRY(fcd_check_launch(who));
   }
-  return dgamma || dbeta ? ln_finish(who, d, a, groups, dgamma, dbeta, accumulate, st) : FCD_OK;
+  return (dgamma || dbeta) && !few ? ln_finish(who, d, a, groups, dgamma, dbeta, accumulate, st) : FCD_OK;
 }
 
