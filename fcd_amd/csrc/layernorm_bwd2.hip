@@ -5,6 +5,9 @@ namespace {
 
 // A row's x, gy and v = ggx in registers; five sums in one exchange, two more if the activation is curved.  With the row's
 // sums in hand gx is a combination of four things: c0 + c1 t + c2 a + c3 xhat (+ rstd q gamma).
+// Bound by memory without an activation, 16384 x 8192 bf16 245 us (5.5 TB/s), 4096 x 4096 29, 65536 x 64 fp32 15.6; with SiLU and
+// dropout by the vector ALU (80 % active at 4096 x 4096 bf16, 40 us).  Four waves a SIMD by force spill: 65536 x 64 fp32 SiLU
+// 17.6 -> 34.6 us.
 // EPI 0: plain; 1: dropout; 2: activation, and dropout if there is any.
 template <typename T, int G, int NV, int EPI>
 __global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd2_rows(LnArgs p) {
@@ -178,6 +181,7 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd2_rows(LnArgs p) {
 }
 
 // Split rows, 1: a chunk's five sums; with the joined ones known and a curved activation (CURVED) the two sums of q gamma.
+// All kernels of a call: 4096 x 12288 bf16 210 us (one workgroup per row that read it again: 489), 8 x 262144 fp32 32.
 template <typename T, int EPI, bool CURVED>
 __global__ __launch_bounds__(256) void ln_bwd2_chunks(LnArgs p, long chunks) {
   constexpr int K = CURVED ? 2 : 5;

@@ -4,8 +4,12 @@
 namespace {
 
 // The row in registers: mean, then the squares around it (two sums: one pass over E[x^2] - mean^2 would lose the spread of
-// rows far from zero), then the result.  A workgroup walks over rows with its columns' parameters in registers and the next
-// row's loads in flight.
+// rows far from zero), then the result.  A workgroup walks over rows with its columns' parameters in registers (fp32 gamma and
+// beta are four times a bf16 row) and the next row's loads in flight; the grid is eight waves a SIMD (half of it: 8192 x 2048
+// bf16 dropout 22.7 -> 23.8 us, 65536 x 1024 plain 42.8 -> 44.7).
+// Bound by memory: 16384 x 8192 bf16 95 us (5.6 TB/s; a large copy runs at 5.1), with dropout 97; 4096 x 4096 14.0, with SiLU
+// and dropout 19.4; 65536 x 64 fp32 8.7, with leaky ReLU and dropout 10.1.  16384 x 8192 with dropout and a residual takes 23
+// vector instructions an element, most of them the generator's.
 template <typename T, int G, int NV, bool EPI>
 __global__ __launch_bounds__(G > 64 ? G : 256) void ln_fwd_rows(LnArgs p) {
   constexpr int TH = G > 64 ? G : 256, RPB = TH / G, WAVES = RowSums<G, 1>::WAVES;

@@ -1,7 +1,8 @@
 """Thin Python wrappers over the C ABI: allocate outputs, pass raw pointers.
 
 Every function here launches HIP kernels from libfcd_hip.so on the current
-stream.  Tensors are fp32; "nhwc" tensors are [N, H, W, CP] with CP a multiple
+stream.  Tensors are fp32 unless a function says otherwise (layer norm and
+dropout also take bf16 and fp16); "nhwc" tensors are [N, H, W, CP] with CP a multiple
 of 4 (pad channels are zero).
 """
 from __future__ import annotations
