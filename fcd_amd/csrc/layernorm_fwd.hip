@@ -87,7 +87,10 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_fwd_rows(LnArgs p) {
       s[0] += q;
     }
     RowSums<G, 1>::run(s, sm, turn);
-    const float rstd = __builtin_amdgcn_rsqf(fmaf(s[0], inv, p.eps));
+    // (the instruction takes a subnormal number, which eps = 0 lets through, for zero)
+    const float var = fmaf(s[0], inv, p.eps);
+    const bool tiny = var < 0x1p-126f;
+    const float rstd = __builtin_amdgcn_rsqf(tiny ? var * 0x1p24f : var) * (tiny ? 0x1p12f : 1.f);
     if (lane == 0 && here && p.mean) {
       p.mean[row] = mean;
       p.rstd[row] = rstd;

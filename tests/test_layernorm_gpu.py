@@ -258,6 +258,24 @@ def test_rows_without_spread(dev, cols):
     R.check(y, wy)
 
 
+@pytest.mark.parametrize("cols", [5, 64, 200, 1001, 8192, 20000])
+def test_tiny_variance_without_eps(dev, cols):
+    """eps 0 and rows whose variance is a subnormal number (about 2^-128).  A square added to a partial sum, and the sum over
+    the length, are off by up to half a step of the subnormal numbers each, 2^-150: the mean of the squares by 2^-149."""
+    from fcd_amd import ops
+    g = torch.Generator().manual_seed(cols)
+    x = (torch.randn(7, cols, generator=g) * 2.0 ** -64).to(dev)
+    w = (1 + 0.2 * torch.randn(cols, generator=g)).to(dev)
+    y, mean, rstd = ops.layernorm_fwd(x, w, None, eps=0.0)
+    d = x.double().cpu()
+    var = ((d - d.mean(1, keepdim=True)) ** 2).mean(1, keepdim=True)
+    assert bool((var < 2.0 ** -126).all()) and bool((var > 2.0 ** -132).all())
+    more = 0.5 * 2.0 ** -149 / var
+    wy, _, wr = R.forward(d, w.double().cpu(), torch.zeros(cols, dtype=torch.float64), 0.0, 1.0, None, None)
+    R.check(rstd, R.V(wr.v, wr.e + more * wr.v), what="rstd")
+    R.check(y, R.V(wy.v, wy.e + more * wy.v.abs()), what="y")
+
+
 def test_dropped_elements_are_zero_whatever_they_held(dev):
     from fcd_amd import ops
     rows, cols, p = 6, 104, 0.5
