@@ -83,6 +83,7 @@ extern "C" int fcd_dropout(const void* x, const void* residual, void* y, int64_t
   if (residual) FCD_TRY(fcd_check_rows(who, vr, rows, cols, es, false));
   FCD_TRY(fcd_check_apart(who, vy, vx, rows, cols, es, true));
   FCD_TRY(fcd_check_apart(who, vy, vr, rows, cols, es, true));
+  FCD_TRY(fcd_check_apart(who, Bytes{"rng", rng, 16}, vy, rows, cols, es));
   if (rows == 0 || cols == 0) return FCD_OK;
   // a tensor without gaps is one long row: no division by the row length, no short ends
   if (rows > 1 && ld_x == cols && ld_y == cols && (!residual || ld_res == cols)) {

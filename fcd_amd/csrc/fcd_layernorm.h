@@ -20,6 +20,9 @@ int ln_check_vectors(const char* who, const FcdLayerNormDesc* d, const void* gam
                      const void* rstd);
 int ln_check_scratch(const char* who, const FcdLayerNormDesc* d, int pass, const void* dgamma, const void* dbeta, void* workspace,
                      size_t workspace_bytes, LnArgs* a);
+// the written vectors w[nw] share memory with nothing: not with one another, the read ones r[nr] or the row tensors t[nt]
+int ln_check_apart(const char* who, const FcdLayerNormDesc* d, const Bytes* w, int nw, const Bytes* r, int nr, const RowView* t,
+                   int nt);
 int ln_finish(const char* who, const FcdLayerNormDesc* d, const LnArgs& a, int groups, void* dgamma, void* dbeta, int accumulate,
               hipStream_t st);
 int ln_groups(int64_t rows, int64_t cols);   // workgroups (row groups of split rows) of the backward passes

@@ -156,6 +156,32 @@ static inline int fcd_check_apart(const char* who, const RowView& out, const Row
   return FCD_EINVAL;
 }
 
+// A vector or scratch that a call writes shares no byte with anything else of the call: workgroups run in any order.
+struct Bytes {
+  const char* name;
+  const void* p;
+  int64_t n;
+};
+
+static inline int fcd_check_apart(const char* who, const Bytes& a, const Bytes& b) {
+  if (!a.p || !b.p || a.n <= 0 || b.n <= 0) return FCD_OK;
+  const __int128 pa = (uintptr_t)a.p, pb = (uintptr_t)b.p;
+  if (pa + a.n <= pb || pb + b.n <= pa) return FCD_OK;
+  fcd_set_error("%s: %s overlaps %s", who, a.name, b.name);
+  return FCD_EINVAL;
+}
+
+// ... with the elements of a row tensor (the gaps between its rows are free)
+static inline int fcd_check_apart(const char* who, const Bytes& a, const RowView& v, int64_t rows, int64_t cols, int esize) {
+  if (!a.p || !v.p || a.n <= 0 || rows <= 0 || cols <= 0) return FCD_OK;
+  const __int128 lo = (__int128)(uintptr_t)a.p - (__int128)(uintptr_t)v.p, row = (__int128)cols * esize;
+  const __int128 pitch = (__int128)(rows > 1 ? v.ld : 0) * esize;
+  if (lo + a.n <= 0 || lo >= pitch * (rows - 1) + row) return FCD_OK;
+  if (pitch > row && lo >= 0 && lo % pitch >= row && lo % pitch + a.n <= pitch) return FCD_OK;
+  fcd_set_error("%s: %s overlaps %s", who, a.name, v.name);
+  return FCD_EINVAL;
+}
+
 #define FCD_TRY(call)            \
   do {                           \
     const int rc_ = (call);      \

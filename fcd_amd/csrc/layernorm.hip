@@ -136,6 +136,17 @@ int ln_check_vectors(const char* who, const FcdLayerNormDesc* d, const void* gam
   return FCD_OK;
 }
 
+int ln_check_apart(const char* who, const FcdLayerNormDesc* d, const Bytes* w, int nw, const Bytes* r, int nr, const RowView* t,
+                   int nt) {
+  const int es = fcd_dt_bytes(d->dtype);
+  for (int i = 0; i < nw; ++i) {
+    for (int k = i + 1; k < nw; ++k) FCD_TRY(fcd_check_apart(who, w[i], w[k]));
+    for (int k = 0; k < nr; ++k) FCD_TRY(fcd_check_apart(who, w[i], r[k]));
+    for (int k = 0; k < nt; ++k) FCD_TRY(fcd_check_apart(who, w[i], t[k], d->rows, d->cols, es));
+  }
+  return FCD_OK;
+}
+
 extern "C" int fcd_layernorm_desc_bytes(void) { return (int)sizeof(FcdLayerNormDesc); }
 
 extern "C" size_t fcd_layernorm_workspace_bytes(const FcdLayerNormDesc* d, int pass, int affine) {

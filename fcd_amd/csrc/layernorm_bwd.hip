@@ -365,6 +365,12 @@ extern "C" int fcd_layernorm_bwd(const FcdLayerNormDesc* d, const void* gy, cons
   FCD_TRY(ln_check_vectors(who, d, gamma, beta, mean, rstd));
   FCD_REQUIRE(d->rows == 0 || (mean && rstd), "%s: mean / rstd are NULL", who);
   FCD_TRY(ln_check_scratch(who, d, FCD_LN_BWD, dgamma, dbeta, workspace, workspace_bytes, &a));
+  const int64_t ps = fcd_dt_bytes(d->param_dtype) * d->cols, ss = 4 * d->rows;
+  const Bytes written[] = {{"dgamma", dgamma, ps}, {"dbeta", dbeta, ps}, {"workspace", workspace, (int64_t)workspace_bytes}};
+  const Bytes read[] = {{"mean", mean, ss}, {"rstd", rstd, ss}, {"gamma", gamma, ps}, {"beta", beta, ps}, {"rng", d->rng, 16}};
+  const RowView rows[] = {vx, vg, vo};
+  FCD_TRY(ln_check_apart(who, d, written, 3, read, 5, rows, 3));
+  for (const Bytes& b : read) FCD_TRY(fcd_check_apart(who, b, vo, d->rows, d->cols, es));
   a.x = x, a.gy = gy, a.gamma = gamma, a.beta = beta, a.out = dx, a.mean = (float*)mean, a.rstd = (float*)rstd;
   const int groups = ln_groups(d->rows, d->cols);
   hipStream_t st = fcd_stream(stream);

@@ -339,6 +339,13 @@ extern "C" int fcd_layernorm_bwd2(const FcdLayerNormDesc* d, const void* ggx, co
   FCD_TRY(ln_check_vectors(who, d, gamma, beta, mean, rstd));
   FCD_REQUIRE(d->rows == 0 || (mean && rstd), "%s: mean / rstd are NULL", who);
   FCD_TRY(ln_check_scratch(who, d, FCD_LN_BWD2, dgamma, dbeta, workspace, workspace_bytes, &a));
+  const int64_t ps = fcd_dt_bytes(d->param_dtype) * d->cols, ss = 4 * d->rows;
+  const Bytes written[] = {{"dgamma", dgamma, ps}, {"dbeta", dbeta, ps}, {"workspace", workspace, (int64_t)workspace_bytes}};
+  const Bytes read[] = {{"mean", mean, ss}, {"rstd", rstd, ss}, {"gamma", gamma, ps}, {"beta", beta, ps}, {"rng", d->rng, 16}};
+  const RowView rows[] = {in[0], in[1], in[2], out[0], out[1]};
+  FCD_TRY(ln_check_apart(who, d, written, 3, read, 5, rows, 5));
+  for (const Bytes& b : read)
+    for (const RowView& v : out) FCD_TRY(fcd_check_apart(who, b, v, d->rows, d->cols, es));
   a.x = x, a.gy = gy, a.ggx = ggx, a.gamma = gamma, a.beta = beta, a.out = gx, a.ggy = ggy;
   a.mean = (float*)mean, a.rstd = (float*)rstd;
   const int groups = ln_groups(d->rows, d->cols);

@@ -272,6 +272,12 @@ extern "C" int fcd_layernorm_fwd(const FcdLayerNormDesc* d, const void* x, const
   FCD_TRY(ln_check_vectors(who, d, gamma, beta, mean, rstd));
   FCD_REQUIRE(!mean == !rstd, "%s: mean and rstd go together", who);
   FCD_TRY(ln_check_scratch(who, d, FCD_LN_FWD, nullptr, nullptr, workspace, workspace_bytes, &a));
+  const int64_t ps = fcd_dt_bytes(d->param_dtype) * d->cols, ss = 4 * d->rows;
+  const Bytes written[] = {{"mean", mean, ss}, {"rstd", rstd, ss}, {"workspace", workspace, (int64_t)workspace_bytes}};
+  const Bytes read[] = {{"gamma", gamma, ps}, {"beta", beta, ps}, {"rng", d->rng, 16}};
+  const RowView rows[] = {vx, vr, vy};
+  FCD_TRY(ln_check_apart(who, d, written, 3, read, 3, rows, 3));
+  for (const Bytes& b : read) FCD_TRY(fcd_check_apart(who, b, vy, d->rows, d->cols, es));
   if (d->rows == 0) return FCD_OK;
   a.x = x, a.gamma = gamma, a.beta = beta, a.res = residual, a.out = y, a.mean = mean, a.rstd = rstd;
   hipStream_t st = fcd_stream(stream);

@@ -484,7 +484,7 @@ int fcd_threshold_hist(const float* diff, const uint8_t* target, size_t n, const
  * gamma / beta / dgamma / dbeta are vectors of `cols` elements of type `param_dtype` (FCD_DT_F32, or the same as
  * `dtype`); mean / rstd are fp32 vectors of `rows`.  All sums are fp32, rounded to the element type once at the end.
  * An output may be the same tensor (address and row stride) as an input of the element type; any other overlap between
- * them is refused.
+ * them is refused, as is a vector or a workspace that is written and shares memory with anything else of the call.
  *
  * Dropout: element i of the rows x cols matrix, i = row * cols + col, takes the 16 bits number i % 8 (low half of word 0
  * first) of block offset + i / 8 of Philox4x32-10 keyed with `seed` (Salmon, Moraes, Dror, Shaw: "Parallel random

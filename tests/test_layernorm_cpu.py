@@ -152,6 +152,55 @@ def test_backward_operands_refused():
             "workspace", -2)
 
 
+def test_vectors_that_share_memory_refused():
+    """A vector or workspace that a call writes shares no byte with anything else of it; gaps between rows are free."""
+    from fcd_amd import _lib
+    lib = _lib.load()
+    f = lambda i: P * 64 * i
+    d = C.byref(desc())                                                  # 4 rows of 16 fp32
+    def fwd(**k):
+        at = {**dict(x=f(1), gamma=f(2), beta=f(3), res=f(4), y=f(5), mean=f(6), rstd=f(7)), **k}
+        return lib.fcd_layernorm_fwd(d, *at.values(), None, 0, None)
+
+    def bwd(d=d, **k):
+        at = {**dict(gy=f(1), x=f(2), mean=f(3), rstd=f(4), gamma=f(5), beta=f(6), dx=f(7), dgamma=f(8), dbeta=f(9)), **k}
+        return lib.fcd_layernorm_bwd(d, *at.values(), 0, None, 0, None)
+
+    def bwd2(**k):
+        at = {**dict(ggx=f(10), gy=f(1), x=f(2), mean=f(3), rstd=f(4), gamma=f(5), beta=f(6), ggy=f(7), gx=f(11), dgamma=f(8),
+                     dbeta=f(9)), **k}
+        return lib.fcd_layernorm_bwd2(d, *at.values(), 0, f(12), lib.fcd_layernorm_workspace_bytes(d, 2, 1), None)
+
+    refused(fwd(rstd=f(6)), "mean overlaps rstd")
+    refused(fwd(rstd=f(6) + 12), "mean overlaps rstd")
+    refused(fwd(mean=f(2) + 60), "mean overlaps gamma")
+    refused(fwd(rstd=f(3) - 12), "rstd overlaps beta")
+    refused(fwd(mean=f(1)), "mean overlaps x")
+    refused(fwd(rstd=f(4) + 255 // 4 * 4), "rstd overlaps residual")
+    refused(fwd(mean=f(5) - 4), "mean overlaps y")
+    refused(fwd(gamma=f(5)), "gamma overlaps y")
+    wide = C.byref(desc(ld_x=24, ld_out=16))
+    refused(lib.fcd_layernorm_fwd(wide, f(1), None, None, None, f(5), f(1) + 64 + 20, f(7), None, 0, None), "mean overlaps x")
+
+    refused(bwd(dgamma=f(9)), "dgamma overlaps dbeta")
+    refused(bwd(dgamma=f(5)), "dgamma overlaps gamma")
+    refused(bwd(dbeta=f(6) + 60), "dbeta overlaps beta")
+    refused(bwd(dbeta=f(3)), "dbeta overlaps mean")
+    refused(bwd(dgamma=f(7)), "dgamma overlaps dx")
+    refused(bwd(dgamma=f(1)), "dgamma overlaps gy")
+    refused(bwd(mean=f(7)), "mean overlaps dx")
+    many = desc(rows=400)
+    need = lib.fcd_layernorm_workspace_bytes(C.byref(many), 1, 1)
+    refused(lib.fcd_layernorm_bwd(C.byref(many), f(1), f(2), f(3), f(4), f(5), f(6), f(7), f(8), f(9), 0, f(8) - 64, need, None),
+            "dgamma overlaps workspace")
+    refused(bwd2(dbeta=f(10)), "dbeta overlaps ggx")
+    refused(bwd2(dgamma=f(11)), "dgamma overlaps gx")
+    refused(bwd2(rstd=f(7) + 4), "rstd overlaps ggy")
+    rng = C.byref(desc(drop_p=0.5, rng=f(7) + 8))
+    refused(bwd(d=rng), "rng overlaps dx")
+    refused(lib.fcd_dropout(f(1), None, f(2), 4, 16, 16, 0, 16, 0, 0.5, 0, 0, f(2) + 248, None), "rng overlaps y")
+
+
 def test_dropout_refused():
     from fcd_amd import _lib
     lib = _lib.load()
