@@ -60,10 +60,9 @@ __global__ __launch_bounds__(256) void dropout_kernel(const T* x, const T* res, 
 }
 
 __global__ void dropout_take_kernel(uint64_t* state, uint64_t* taken, uint64_t blocks) {
-  const uint64_t seed = state[0], offset = state[1];
-  taken[0] = seed;
-  taken[1] = offset;
-  state[1] = offset + blocks;
+  // (an atomic: calls on two streams at once take two ranges)
+  taken[0] = state[0];
+  taken[1] = atomicAdd((unsigned long long*)state + 1, (unsigned long long)blocks);
 }
 
 }  // namespace

@@ -546,7 +546,8 @@ int fcd_dropout(const void* x, const void* residual, void* y, int64_t rows, int6
                 int64_t ld_y, int dtype, double drop_p, uint64_t seed, uint64_t offset, const uint64_t* rng,
                 void* stream);
 /* taken[0..1] = state[0..1], then state[1] += blocks (device words): hands out a range of blocks of the generator, also
- * inside a captured graph.  Rows * cols elements use (rows * cols + 7) / 8 blocks. */
+ * inside a captured graph; calls that run at once take different ranges.  Rows * cols elements use
+ * (rows * cols + 7) / 8 blocks. */
 int fcd_dropout_take(uint64_t* state, uint64_t* taken, uint64_t blocks, void* stream);
 
 #ifdef __cplusplus

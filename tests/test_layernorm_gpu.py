@@ -371,6 +371,41 @@ def _step(ops, t, rng, gb):
     return [y, mean, rstd, dx, dg, db, *o2, z]
 
 
+def test_taking_ranges_on_two_streams(dev):
+    """Every block is handed out once, whichever stream asks first."""
+    from fcd_amd import ops
+    state = ops.dropout_state(11, dev)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    taken = []
+    torch.cuda.synchronize()
+    for i in range(200):
+        with torch.cuda.stream(streams[i % 2]):
+            taken.append(ops.dropout_take(state, 24))
+    torch.cuda.synchronize()
+    assert sorted(int(t[1]) for t in taken) == [3 * i for i in range(200)]
+    assert all(int(t[0]) == 11 for t in taken) and state.tolist() == [11, 600]
+
+
+def test_statistics_between_rows(dev):
+    """mean and rstd may lie in the gap behind a row of a wider tensor."""
+    import ctypes as C
+    from fcd_amd import _lib, ops
+    t, _ = case(dev, 4, 40, F32)
+    wide = torch.zeros(4, 56, device=dev)
+    wide[:, :40] = t["x"]
+    y = torch.empty(4, 40, device=dev)
+    d = _lib.LayerNormDesc()
+    for k, v in dict(rows=4, cols=40, ld_x=56, ld_out=40, eps=ops.LN_EPS, act=1.0).items():
+        setattr(d, k, v)
+    at = wide.data_ptr() + (56 + 40) * 4
+    rc = _lib.load().fcd_layernorm_fwd(C.byref(d), wide.data_ptr(), t["gamma"].data_ptr(), t["beta"].data_ptr(), None, y.data_ptr(),
+                                       at, at + 16, None, 0, _lib.stream())
+    _lib.check(rc, "layernorm_fwd")
+    wy, wm, wr = ops.layernorm_fwd(t["x"].contiguous(), t["gamma"], t["beta"])
+    assert torch.equal(y, wy) and torch.equal(wide[1, 40:44], wm) and torch.equal(wide[1, 44:48], wr)
+    assert torch.equal(wide[:, :40], t["x"])
+
+
 @pytest.mark.parametrize("rows,cols", [(700, 64), (300, 1000), (40, 9000)])
 def test_captured_graphs(dev, rows, cols):
     """Two graphs of the same step, replayed in turn with eager work between: every replay draws the next masks and gives the
