@@ -84,6 +84,7 @@ __device__ __forceinline__ void drop_draw8(const Drop& d, uint64_t i, uint32_t (
   const uint32_t phase = (uint32_t)i & 7u;
   drop_block(d, block, w);
   if (phase) {
+    asm volatile("");                    // (a branch: without it the compiler draws both blocks always and selects)
     uint32_t n[4];
     drop_block(d, block + 1, n);
     // the two blocks as eight words, moved down by `phase` halves (scalars: an array would be indexed in memory)

@@ -5,8 +5,8 @@ namespace {
 
 // The row in registers: mean, then the squares around it (two sums: one pass over E[x^2] - mean^2 would lose the spread of
 // rows far from zero), then the result.  A workgroup walks over rows with its columns' parameters in registers (fp32 gamma and
-// beta are four times a bf16 row) and the next row's loads in flight; the grid is eight waves a SIMD (half of it: 8192 x 2048
-// bf16 dropout 22.7 -> 23.8 us, 65536 x 1024 plain 42.8 -> 44.7).
+// beta are four times a bf16 row) and the next row's loads in flight; the grid is eight waves a SIMD (half of it: 65536 x 1024
+// bf16 42.8 -> 44.7 us), or one workgroup of 1024, of which no second one fits (2048 x 12288 bf16 dropout with two 28.6, 26.4).
 // Bound by memory: 16384 x 8192 bf16 95 us (5.6 TB/s; a large copy runs at 5.1), with dropout 97; 4096 x 4096 14.0, with SiLU
 // and dropout 19.4; 65536 x 64 fp32 8.7, with leaky ReLU and dropout 10.1.  16384 x 8192 with dropout and a residual takes 23
 // vector instructions an element, most of them the generator's.
@@ -240,7 +240,7 @@ void launch(const LnArgs& a, hipStream_t st) {
 #define SHAPE(G, NV)                                                        \
   if (units <= G * NV) {                                                    \
     const int th = G > 64 ? G : 256;                                        \
-    const long need = (a.rows + th / G - 1) / (th / G), full = 256 * (2048 / th); \
+    const long need = (a.rows + th / G - 1) / (th / G), full = 256 * (G == 1024 ? 1 : 2048 / th); \
     const unsigned grid = (unsigned)(need < full ? need : full);            \
     if (epi) ln_fwd_rows<T, G, NV, true><<<grid, th, 0, st>>>(a);           \
     else ln_fwd_rows<T, G, NV, false><<<grid, th, 0, st>>>(a);              \
