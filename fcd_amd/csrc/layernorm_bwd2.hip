@@ -6,7 +6,7 @@ namespace {
 // A row's x, gy and v = ggx in registers; five sums in one exchange, two more if the activation is curved.  With the row's
 // sums in hand gx is a combination of four things: c0 + c1 t + c2 a + c3 xhat (+ rstd q gamma).
 // Bound by memory without an activation, 16384 x 8192 bf16 245 us (5.5 TB/s), 4096 x 4096 29, 65536 x 64 fp32 15.6; with SiLU and
-// dropout by the vector ALU (80 % active at 4096 x 4096 bf16, 40 us).  Four waves a SIMD by force spill: 65536 x 64 fp32 SiLU
+// dropout by the vector ALU (81 % active at 4096 x 4096 bf16, 40 us).  Four waves a SIMD by force spill: 65536 x 64 fp32 SiLU
 // 17.6 -> 34.6 us.
 // EPI 0: plain; 1: dropout; 2: activation, and dropout if there is any.
 template <typename T, int G, int NV, int EPI>
