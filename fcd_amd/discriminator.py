@@ -84,12 +84,12 @@ class Discriminator(_Drops):
 
     Beyond the reference: ``norm="layer"`` puts a layer norm over the channels of each pixel between every strided
     convolution and its activation (parameters ``*.1.{weight,bias}``; a critic under a gradient penalty cannot take a norm
-    that couples samples), ``dropout`` drops activations in training mode (``dropout_seed``: None takes torch's initial
-    seed; the generator's state is a buffer).  Off by default."""
+    that couples samples), ``dropout`` drops activations in training mode (``dropout_seed``: None draws one from
+    torch's generator; the generator's state is a buffer).  Off by default."""
 
     def __init__(self, image_size=128, conv_dim=64, c_dim=5, repeat_num=6, num_channels=3, activation="lrelu",
                  n_feature_layers=4, interm_non_act=False, use_attention=False, norm="none", dropout=0.0, dropout_seed=None):
-        super().__init__(dropout, dropout_seed)
+        super().__init__(dropout)
         if norm not in ("none", "layer"):
             raise NotImplementedError(f"discriminator norm {norm!r} has no HIP path")
         if interm_non_act and (norm != "none" or dropout > 0.0):
@@ -146,6 +146,7 @@ class Discriminator(_Drops):
         self.merge_wgrad = os.environ.get("FCD_MERGE_WGRAD_D", os.environ.get("FCD_MERGE_WGRAD", "1")) != "0"
         self._pairing = ops.WgradPairing()
         self._wmax = WeightMaxima(self._convs)     # max |weight| of the six layers in one launch per optimizer step
+        self._start(dropout_seed)                  # (last: the parameters are those of a critic without dropout)
 
     def _flat_params(self):
         out = []

@@ -116,15 +116,24 @@ def rank_offset() -> int:
 
 
 class _Drops(nn.Module):
-    """Dropout probability and the generator's state (a buffer: it moves with the module and resumes from a checkpoint)."""
+    """Dropout probability and the generator's state (a buffer: it moves with the module and resumes from a checkpoint).
 
-    def __init__(self, p: float, seed: Optional[int]):
+    Without a seed a module draws one from torch's CPU generator, so every module has masks of its own and ``manual_seed``
+    brings them back.  Modules that are given one seed, and copies of a module, draw the same blocks: the same masks, for equal
+    shapes."""
+
+    def __init__(self, p: float):
         super().__init__()
         if not 0.0 <= p <= 1.0:
             raise ValueError(f"dropout probability {p} is not in [0, 1]")
         self.p = float(p)
-        if self.p > 0.0:
-            self.register_buffer("dropout_state", ops.dropout_state(torch.initial_seed() if seed is None else seed, "cpu"))
+
+    def _start(self, seed: Optional[int]) -> None:
+        if self.p == 0.0:
+            return
+        if seed is None:
+            seed = int(torch.empty((), dtype=torch.int64, device="cpu").random_())
+        self.register_buffer("dropout_state", ops.dropout_state(seed, "cpu"))
 
     def _draw(self, numel: int):
         """(p, rng) of this call."""
@@ -137,7 +146,8 @@ class Dropout(_Drops):
     """Dropout whose mask is recomputed in the backward pass; the identity in eval mode."""
 
     def __init__(self, p: float = 0.5, seed: Optional[int] = None):
-        super().__init__(p, seed)
+        super().__init__(p)
+        self._start(seed)
 
     def forward(self, x, residual=None):
         p, rng = self._draw(x.numel())
@@ -149,8 +159,9 @@ class LayerNorm(_Drops):
 
     def __init__(self, dim: int, eps: float = ops.LN_EPS, affine: bool = True, bias: bool = True,
                  activation: Optional[str] = None, dropout: float = 0.0, seed: Optional[int] = None):
-        super().__init__(dropout, seed)
+        super().__init__(dropout)
         _code(activation)
+        self._start(seed)
         self.dim, self.eps, self.activation = int(dim), float(eps), activation
         self.weight = nn.Parameter(torch.ones(dim)) if affine else None
         self.bias = nn.Parameter(torch.zeros(dim)) if affine and bias else None

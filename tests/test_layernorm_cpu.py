@@ -287,3 +287,28 @@ def test_modules_refuse_the_cpu_and_bad_arguments():
         Dropout(-0.1)
     with pytest.raises(NotImplementedError):
         LayerNorm(8, activation="tanh")
+
+
+def test_modules_without_a_seed_draw_apart():
+    """Modules whose seed is left out get generators of their own, the same ones again under the same ``manual_seed``; a given
+    seed is taken as it is; parameters come out as without dropout."""
+    from fcd_amd import Discriminator, Dropout, LayerNorm
+
+    def build():
+        torch.manual_seed(12)
+        return [Dropout(0.5), Dropout(0.5), LayerNorm(8, dropout=0.5), LayerNorm(8, dropout=0.5),
+                Discriminator(32, 8, 1, 3, 10, n_feature_layers=2, dropout=0.5)]
+
+    first, again = build(), build()
+    states = [tuple(m.dropout_state.tolist()) for m in first]
+    assert len({s for s, _ in states}) == len(states) and all(o == 0 for _, o in states)
+    assert states == [tuple(m.dropout_state.tolist()) for m in again]
+    assert Dropout(0.5, seed=7).dropout_state.tolist() == LayerNorm(8, dropout=0.1, seed=7).dropout_state.tolist() == [7, 0]
+    torch.manual_seed(5)
+    with_dropout = Discriminator(32, 8, 1, 3, 10, n_feature_layers=2, dropout=0.5)
+    torch.manual_seed(5)
+    without = Discriminator(32, 8, 1, 3, 10, n_feature_layers=2)
+    assert all(torch.equal(a, b) for a, b in zip(with_dropout.parameters(), without.parameters()))
+    before = torch.get_rng_state()
+    Dropout(0.0), LayerNorm(8), Dropout(0.5, seed=1)                # nothing to draw: torch's generator stays where it is
+    assert torch.equal(before, torch.get_rng_state())

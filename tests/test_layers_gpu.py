@@ -315,3 +315,17 @@ def test_training_steps_with_norm_and_dropout(dev, precision):
     state = s.D.dropout_state.clone()
     x = torch.rand(2, 10, 32, 32, device=dev)
     assert torch.equal(s.D(x)[0], s.D(x)[0]) and torch.equal(state, s.D.dropout_state)
+
+
+def test_modules_without_a_seed_drop_other_elements(dev):
+    """Three modules of one model on one shape: each pair of masks agrees where two independent draws would (share 1/2 of 2^16
+    elements within 6 standard deviations), at the first step and at the next."""
+    from fcd_amd import Dropout, LayerNorm
+    torch.manual_seed(3)
+    mods = [Dropout(0.5).to(dev), Dropout(0.5).to(dev), LayerNorm(64, dropout=0.5).to(dev)]
+    x = torch.randn(1024, 64, device=dev) + 5
+    for _ in range(2):
+        kept = [m(x) != 0 for m in mods]
+        for i in range(3):
+            for k in range(i):
+                assert abs(float((kept[i] == kept[k]).double().mean()) - 0.5) <= 6 * (0.25 / x.numel()) ** 0.5
