@@ -235,7 +235,8 @@ __device__ __forceinline__ void idle_sums(float* sm, int& turn) {
 // ---------------------------------------------------------------- activations ----------
 // The smooth ones from one hardware exponential and one hardware reciprocal (a step of fp32 each).  exp(u) as 2^(u log2 e)
 // loses |u| / 2 steps relative; what it is used in changes by at most |u| s (1 - s) < 0.23 times that.
-// mish, e = exp(u), n = e (e + 2): tanh(log(1 + e)) = n / (n + 2), its derivative w = 4 e (1 + e) / (n + 2)^2.
+// mish, e = exp(u), n = e (e + 2): tanh(log(1 + e)) = n / (n + 2), its derivative w = 4 e (1 + e) / (n + 2)^2.  Beyond u = 20
+// that is 1 in fp32 and w below 2e-17, where u itself may be anything: e and the factor of w take u clamped (NaN stays NaN).
 __device__ __forceinline__ float fast_exp(float u) { return __builtin_amdgcn_exp2f(u * 1.44269504088896341f); }
 
 // The activation (d0) of 8 values, or its first (d1) and second (d2) derivative; what is NULL is not computed.
@@ -251,13 +252,14 @@ __device__ __forceinline__ void ln_act8(const float (&u)[8], float code, float* 
   } else if (code == FCD_ACT_MISH) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float e = fast_exp(fminf(u[j], 20.f)), n = e * (e + 2.f), r = __builtin_amdgcn_rcpf(n + 2.f), th = n * r;
+      const float uc = u[j] > 20.f ? 20.f : u[j];
+      const float e = fast_exp(uc), n = e * (e + 2.f), r = __builtin_amdgcn_rcpf(n + 2.f), th = n * r;
       if (d0) d0[j] = u[j] * th;
       const float w = 4.f * e * (1.f + e) * r * r;
-      if (d1) d1[j] = fmaf(u[j], w, th);
+      if (d1) d1[j] = fmaf(uc, w, th);
       if (d2) {
         const float sg = e * __builtin_amdgcn_rcpf(1.f + e);
-        d2[j] = w * fmaf(u[j], (1.f - sg) - 2.f * th * sg, 2.f);
+        d2[j] = w * fmaf(uc, (1.f - sg) - 2.f * th * sg, 2.f);
       }
     }
   } else {

@@ -166,3 +166,34 @@ def backward2(ggx, x, gy, mean, rstd, gamma, beta, code, mask):
     hx = (qg * xh).mean() - vx * ax * rstd * 2.0
     gx = (h - hm - xh * hx) * rstd - s * rstd * rstd * xh
     return ggy, gx, (g1 * t + q * xh).colsum(), q.colsum()
+
+
+def second(ggx, x, gy, mean, rstd, gamma, beta, code, mask, derivatives=None):
+    """:func:`backward2` with every product taken around its means, so that the bounds grow with the operands' offsets and not
+    with their square.  ``derivatives``: act'(u) and act''(u) in place of those of ``code``."""
+    xh = (V(x) - mean) * rstd
+    u = xh * gamma + beta
+    m = V(mask, U * mask) if mask is not None else None
+    g = V(gy) * m if mask is not None else V(gy)
+    d1, d2 = derivatives or (act(u, code, 1), act(u, code, 2))
+    g1 = g * d1
+    a, v = g1 * gamma, V(ggx)
+    am, ax, vm, vx = a.mean(), (a * xh).mean(), v.mean(), (v * xh).mean()
+    ac, w = a - am, v - vm - xh * vx
+    s = (w * ac).mean()
+    t = w * rstd
+    ggy = d1 * gamma * t
+    ggy = ggy * m if mask is not None else ggy
+    q = g * d2 * gamma * t
+    qg = q * gamma
+    # h - mean h - xh mean(h xh) with h = q gamma - rstd (v A + a B) written in w and in a around its mean
+    gx = (qg - qg.mean() - xh * (qg * xh).mean()) * rstd - (w * ax + ac * vx - xh * (ax * vx)) * rstd * rstd - s * rstd * rstd * xh
+    return ggy, gx, (g1 * t + q * xh).colsum(), q.colsum()
+
+
+def first(x, gy, mean, rstd, gamma, d1):
+    """:func:`backward` for a given act'(u)."""
+    xh = (V(x) - mean) * rstd
+    g1 = V(gy) * d1
+    a = g1 * gamma
+    return (a - a.mean() - xh * (a * xh).mean()) * rstd, (g1 * xh).colsum(), g1.colsum()

@@ -312,3 +312,20 @@ def test_modules_without_a_seed_draw_apart():
     before = torch.get_rng_state()
     Dropout(0.0), LayerNorm(8), Dropout(0.5, seed=1)                # nothing to draw: torch's generator stays where it is
     assert torch.equal(before, torch.get_rng_state())
+
+
+@pytest.mark.parametrize("code", [1.0, 0.01, 2.0, 3.0])
+@pytest.mark.parametrize("offset", [0.0, 100.0])
+def test_centred_second_backward_is_the_same_function(code, offset):
+    """The second backward's formula around the means equals the one that is checked against autograd."""
+    g = torch.Generator().manual_seed(6)
+    x, gy, v = (torch.randn(6, 23, generator=g, dtype=torch.float64) + s for s in (0.0, offset, offset))
+    ga, be = 1 + 0.2 * torch.randn(23, generator=g, dtype=torch.float64), 0.2 * torch.randn(23, generator=g, dtype=torch.float64)
+    m = R.keep_mask(6, 23, 0.4, 5, 6)
+    mean = x.mean(1, keepdim=True)
+    rstd = (((x - mean) ** 2).mean(1, keepdim=True) + 1e-5) ** -0.5
+    for got, want in zip(R.second(v, x, gy, mean, rstd, ga, be, code, m), R.backward2(v, x, gy, mean, rstd, ga, be, code, m)):
+        assert torch.allclose(got.v, want.v, rtol=1e-9, atol=1e-9 * max(1.0, offset ** 2))
+    one = R.V(torch.full((6, 23), 0.5, dtype=torch.float64))
+    for got, want in zip(R.first(x, gy, mean, rstd, ga, one), R.backward(x, gy * 0.5, mean, rstd, ga, be, 1.0, None)):
+        assert torch.allclose(got.v, want.v, rtol=1e-12, atol=1e-10)

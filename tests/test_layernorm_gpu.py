@@ -512,3 +512,31 @@ def test_split_rows(dev, rows, cols):
     run_all(dev, rows, cols, F32, 2.0, 0.1)
     run_all(dev, rows, cols, BF16, 1.0, 0.0, pad=3, residual=True)
     run_all(dev, rows, cols, F16, 0.01, 0.4, seed=2)
+
+
+# ---- activations far out ----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("code", [2.0, 3.0])
+@pytest.mark.parametrize("far", [60.0, 1e4, 1e8, 1e12, 1e16, 1e20, 3e30])
+def test_smooth_activations_far_from_zero(dev, code, far):
+    """Pre-activations of +-far (through beta): act is u or 0, act' 1 or 0, act'' 0, within four steps of fp32 however large u
+    is.  (|u| > 50: the exact ones are within 50 e^-50 < 1e-15 of these.)"""
+    from fcd_amd import ops
+    for rows, cols in ((3, 24), (700, 64), (5, 1000), (300, 1537), (3, 9001)):
+        t, d = case(dev, rows, cols, F32)
+        up = torch.rand(cols, generator=torch.Generator().manual_seed(cols)) < 0.5
+        t["beta"] = torch.where(up, far, -far).to(dev)
+        d["beta"] = t["beta"].double().cpu()
+        y, mean, rstd = ops.layernorm_fwd(t["x"], t["gamma"], t["beta"], act_slope=code)
+        wy, _, _ = R.forward(d["x"], d["gamma"], d["beta"], ops.LN_EPS, 1.0, None, None)
+        R.check(y, R.V(wy.v * up, (wy.e + 4 * R.U * wy.v.abs()) * up + 1e-15), what="y")
+        md, rd = mean.double().cpu()[:, None], rstd.double().cpu()[:, None]
+        one = R.V(up.double().expand(rows, cols), 4 * R.U)
+        flat = R.V(torch.zeros(rows, cols, dtype=torch.float64), 1e-15)
+        got = ops.layernorm_bwd(t["gy"], t["x"], mean, rstd, t["gamma"], t["beta"], act_slope=code)
+        for g, w, name in zip(got, R.first(d["x"], d["gy"], md, rd, d["gamma"], one), ("dx", "dgamma", "dbeta")):
+            R.check(g, w, what=name)
+        got = ops.layernorm_bwd2(t["ggx"], t["gy"], t["x"], mean, rstd, t["gamma"], t["beta"], act_slope=code)
+        want = R.second(d["ggx"], d["x"], d["gy"], md, rd, d["gamma"], d["beta"], code, None, (one, flat))
+        for g, w, name in zip(got, want, ("ggy", "gx", "dgamma", "dbeta")):
+            R.check(g, w, what="second " + name)
