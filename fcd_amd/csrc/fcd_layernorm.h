@@ -169,14 +169,14 @@ __device__ __forceinline__ float lane_value(float v, int lane) {
 }
 
 // Sums of K values over the G threads of a row, in every thread (from a wave on in scalar registers).  A wave's sums share
-// their exchanges: each swap folds two of them at once, so that five cost 21 instructions and not 50, and end up in the lanes
-// home(k).  More than a wave: one barrier; `turn` alternates between two buffers, and a wave writes to one again only behind
-// the barrier of the other, which every wave reaches after its reads.
+// their exchanges: each swap folds two of them at once, so that four cost little more than one, and end up in the lanes home(k).
+// More than a wave: one barrier; `turn` alternates between two buffers, and a wave writes to one again only behind the barrier of
+// the other, which every wave reaches after its reads.
 template <int G, int K>
 struct RowSums {
-  static_assert(K == 1 || K == 2 || K == 5, "");
+  static_assert(K >= 1 && K <= 4, "");
   static constexpr int WAVES = G > 64 ? G / 64 : 1;
-  __device__ __forceinline__ static constexpr int home(int k) { return K == 1 ? 0 : K == 2 ? 32 * k : k < 4 ? 32 * (k & 1) + 8 * (k & 2) : 1; }
+  __device__ __forceinline__ static constexpr int home(int k) { return 32 * (k & 1) + 8 * (k & 2); }
 
   __device__ __forceinline__ static float fold(const float (&s)[K]) {
     if constexpr (K == 1) return lanes_sum<64>(s[0]);
@@ -184,10 +184,7 @@ struct RowSums {
       const float r = swap32_add(s[0], s[1]);
       return lanes_sum<16>(swap16_add(r, r));
     }
-    if constexpr (K == 5) {
-      const float r = lanes_sum<16>(swap16_add(swap32_add(s[0], s[1]), swap32_add(s[2], s[3]))), t = lanes_sum<64>(s[4]);
-      return (threadIdx.x & 63) == 1 ? t : r;
-    }
+    if constexpr (K > 2) return lanes_sum<16>(swap16_add(swap32_add(s[0], s[1]), swap32_add(s[2], s[K - 1])));
   }
 
   __device__ __forceinline__ static void run(float (&s)[K], float* sm, int& turn) {
@@ -209,11 +206,10 @@ struct RowSums {
         if (mine >= 0) buf[mine * WAVES + w] = r;
         __syncthreads();
         // sum k's waves in WAVES neighbouring lanes
-        constexpr int FIRST = K * WAVES < 64 ? K * WAVES : 64;
-        const float a = lanes_sum<WAVES>(buf[lane < FIRST ? lane : 0]);
+        static_assert(K * WAVES <= 64, "");
+        const float a = lanes_sum<WAVES>(buf[lane < K * WAVES ? lane : 0]);
 #pragma unroll
-        for (int k = 0; k < K && k * WAVES < 64; ++k) s[k] = lane_value(a, k * WAVES);
-        if constexpr (K * WAVES > 64) s[4] = lane_value(lanes_sum<WAVES>(buf[64 + (lane & (WAVES - 1))]), 0);
+        for (int k = 0; k < K; ++k) s[k] = lane_value(a, k * WAVES);
       }
     }
   }

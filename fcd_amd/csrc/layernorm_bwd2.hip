@@ -3,16 +3,20 @@
 
 namespace {
 
-// A row's x, gy and v = ggx in registers; five sums in one exchange, two more if the activation is curved.  With the row's
-// sums in hand gx is a combination of four things: c0 + c1 t + c2 a + c3 xhat (+ rstd q gamma).
+// A row's x, gy and v = ggx in registers; the four means in one exchange, then S = mean((v - mean v - xhat mean(v xhat)) (a -
+// mean a)) and behind a curved activation the two sums of q gamma in a second one.  (S in the first exchange, as mean(v a) less
+// the products of the means, loses the square of the gradients' offsets.  The second exchange costs 0 to 3 %; 4096 x 4095 40 ->
+// 44 us, 2048 x 8192 behind a leaky slope 37.7 -> 39.7.  Waves that centre on their own means and join them in the first one:
+// equal or slower, and spilt.)
+// With the row's sums in hand gx is a combination of four things: c0 + c1 t + c2 a + c3 xhat (+ rstd q gamma).
 // Bound by memory without an activation, 16384 x 8192 bf16 245 us (5.5 TB/s), 4096 x 4096 29, 65536 x 64 fp32 15.6; with SiLU and
 // dropout by the vector ALU (81 % active at 4096 x 4096 bf16, 40 us).  Four waves a SIMD by force spill: 65536 x 64 fp32 SiLU
 // 17.6 -> 34.6 us.
 // EPI 0: plain; 1: dropout; 2: activation, and dropout if there is any.
 template <typename T, int G, int NV, int EPI>
 __global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd2_rows(LnArgs p) {
-  constexpr int TH = G > 64 ? G : 256, RPB = TH / G, WAVES = RowSums<G, 5>::WAVES;
-  __shared__ float sm[2 * 5 * WAVES], sm2[2 * 2 * WAVES];
+  constexpr int TH = G > 64 ? G : 256, RPB = TH / G, WAVES = RowSums<G, 4>::WAVES;
+  __shared__ float sm[2 * 4 * WAVES], sm2[2 * (EPI == 2 ? 3 : 1) * WAVES];
   __shared__ float aff[affine_lds<G, NV>()];
   int turn = 0, turn2 = 0;
   if (EPI) drop_state(p.drop);
@@ -51,8 +55,9 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd2_rows(LnArgs p) {
   long turns = (p.rows - (G >= 64 ? row : (long)blockIdx.x * RPB) + step - 1) / step;
   if (idle_wave<G>(cols)) {
     for (; turns > 0; --turns) {
-      idle_sums<G, 5>(sm, turn);
-      if (curved) idle_sums<G, 2>(sm2, turn2);
+      idle_sums<G, 4>(sm, turn);
+      if (curved) idle_sums<G, 3>(sm2, turn2);
+      else idle_sums<G, 1>(sm2, turn2);
     }
   }
   // a workgroup of 1024 has 128 registers a thread: behind an activation they do not hold the next row as well
@@ -70,7 +75,7 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd2_rows(LnArgs p) {
     if (!AHEAD) fetch(row);
     const float mean = nmean, rstd = nrstd;
     // xhat, drop(gy), v, and behind an activation act'(u) and act''(u)
-    float xh[NV][8], g[NV][8], v[NV][8], d1[NV][8], q[NV][8], s[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
+    float xh[NV][8], g[NV][8], v[NV][8], d1[NV][8], q[NV][8], s[4] = {0.f, 0.f, 0.f, 0.f};
     uint32_t w[NV][4];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
@@ -102,7 +107,7 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd2_rows(LnArgs p) {
           g[k][j] *= d1[k][j];                        // g1
         }
       }
-      float t[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
+      float t[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float a = g[k][j] * ga[k][j];
@@ -110,39 +115,49 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd2_rows(LnArgs p) {
         t[1] = fmaf(a, xh[k][j], t[1]);
         t[2] += v[k][j];
         t[3] = fmaf(v[k][j], xh[k][j], t[3]);
-        t[4] = fmaf(v[k][j], a, t[4]);
       }
 #pragma unroll
-      for (int i = 0; i < 5; ++i) s[i] += t[i];
+      for (int i = 0; i < 4; ++i) s[i] += t[i];
     }
-    RowSums<G, 5>::run(s, sm, turn);
+    RowSums<G, 4>::run(s, sm, turn);
     const float am = s[0] * inv, ax = s[1] * inv, vm = s[2] * inv, vx = s[3] * inv;
-    const float sv = s[4] * inv - vm * am - vx * ax;
     // t, the cotangent of a, in the place of v
+    float ts = 0.f, q0 = 0.f, q1 = 0.f;
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
+    for (int k = 0; k < NV; ++k) {
+      const int n = cols - (lane + k * G) * 8;
+      float ac[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[k][j] = rstd * (v[k][j] - vm - xh[k][j] * vx);
-    float q2[2] = {0.f, 0.f};
-    if (EPI == 2 && curved) {
+      for (int j = 0; j < 8; ++j) ac[j] = fmaf(g[k][j], ga[k][j], -am);
+      if (n < 8) {
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        float q0 = 0.f, q1 = 0.f;
+        for (int j = 0; j < 8; ++j) ac[j] = j < n ? ac[j] : 0.f;
+      }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < 8; ++j) {
+        const float w = v[k][j] - vm - xh[k][j] * vx;
+        ts = fmaf(w, ac[j], ts);
+        v[k][j] = rstd * w;
+        if (EPI == 2) {
           q[k][j] *= v[k][j];
           const float qg = q[k][j] * ga[k][j];
           q0 += qg;
           q1 = fmaf(qg, xh[k][j], q1);
         }
-        q2[0] += q0;
-        q2[1] += q1;
       }
-      RowSums<G, 2>::run(q2, sm2, turn2);
+    }
+    if (EPI == 2 && curved) {
+      float s2[3] = {ts, q0, q1};
+      RowSums<G, 3>::run(s2, sm2, turn2);
+      ts = s2[0], q0 = s2[1], q1 = s2[2];
+    } else {
+      float s2[1] = {ts};
+      RowSums<G, 1>::run(s2, sm2, turn2);
+      ts = s2[0];
     }
     // with v = t / rstd + mean(v) + xhat mean(v xhat) put into h:
-    const float c0 = rstd * (rstd * am * vx - q2[0] * inv), c1 = -rstd * ax, c2 = -rstd * rstd * vx;
-    const float c3 = -rstd * (q2[1] * inv + rstd * (sv - vx * ax));
+    const float c0 = rstd * (rstd * am * vx - q0 * inv), c1 = -rstd * ax, c2 = -rstd * rstd * vx;
+    const float c3 = -rstd * (q1 * inv + rstd * (ts * inv - vx * ax));
     T *ggy = (T*)p.ggy + row * p.ld_ggy, *out = (T*)p.out + row * p.ld_out;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
@@ -180,13 +195,14 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd2_rows(LnArgs p) {
   if (p.partial) write_partial<G, NV>(p, dg, db, aff);
 }
 
-// Split rows, 1: a chunk's five sums; with the joined ones known and a curved activation (CURVED) the two sums of q gamma.
+// Split rows, 1: a chunk's sums of a, a xhat, v and v xhat, and that of (v - its mean) (a - its mean) around the chunk's own
+// means; with the joined ones known and a curved activation (CURVED) the two sums of q gamma.
 // All kernels of a call: 4096 x 12288 bf16 210 us (one workgroup per row that read it again: 489), 8 x 262144 fp32 32.
 template <typename T, int EPI, bool CURVED>
 __global__ __launch_bounds__(256) void ln_bwd2_chunks(LnArgs p, long chunks) {
   constexpr int K = CURVED ? 2 : 5;
-  __shared__ float sm[2 * K * 4];
-  int turn = 0;
+  __shared__ float sm[2 * 4 * 4], sm2[2 * 4];
+  int turn = 0, turn2 = 0;
   if (EPI) drop_state(p.drop);
   const float inv = 1.f / (float)p.cols;
   for (long item = blockIdx.x; item < p.rows * chunks; item += gridDim.x) {
@@ -194,45 +210,78 @@ __global__ __launch_bounds__(256) void ln_bwd2_chunks(LnArgs p, long chunks) {
     const T *x = (const T*)p.x + row * p.ld_x, *gy = (const T*)p.gy + row * p.ld_gy, *ggx = (const T*)p.ggx + row * p.ld_ggx;
     const float mean = p.mean[row], rstd = p.rstd[row];
     const float vm = CURVED ? p.row[row * ROW_SUMS + 2] * inv : 0.f, vx = CURVED ? p.row[row * ROW_SUMS + 3] * inv : 0.f;
-    float s[K];
-#pragma unroll
-    for (int i = 0; i < K; ++i) s[i] = 0.f;
+    float s[CURVED ? 2 : 4] = {}, a[4][8], v[4][8];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int c = (int)c0 + (threadIdx.x + k * 256) * 8, n = (int)p.cols - c;
       Eight<EPI, CURVED> e;
-      float ga[8], be[8], v[8];
+      float ga[8], be[8];
       load8(x + c, n, e.xh);
       load8(gy + c, n, e.g);
-      load8(ggx + c, n, v);
+      load8(ggx + c, n, v[k]);
       load_param<T>(p.gamma, p.param_f32, c, n, 1.f, ga);
       if (EPI == 2) load_param<T>(p.beta, p.param_f32, c, n, 0.f, be);
       e.make(p, row, c, mean, rstd, ga, be);
-      float t[K];
-#pragma unroll
-      for (int i = 0; i < K; ++i) t[i] = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         if constexpr (CURVED) {
-          const float qg = e.g[j] * e.d2[j] * ga[j] * (rstd * (v[j] - vm - e.xh[j] * vx)) * ga[j];
-          t[0] += qg;
-          t[1] = fmaf(qg, e.xh[j], t[1]);
+          const float qg = e.g[j] * e.d2[j] * ga[j] * (rstd * (v[k][j] - vm - e.xh[j] * vx)) * ga[j];
+          s[0] += qg;
+          s[1] = fmaf(qg, e.xh[j], s[1]);
         } else {
-          const float a = (EPI == 2 ? e.g[j] * e.d1[j] : e.g[j]) * ga[j];
-          t[0] += a;
-          t[1] = fmaf(a, e.xh[j], t[1]);
-          t[2] += v[j];
-          t[3] = fmaf(v[j], e.xh[j], t[3]);
-          t[4] = fmaf(v[j], a, t[4]);
+          a[k][j] = (EPI == 2 ? e.g[j] * e.d1[j] : e.g[j]) * ga[j];
+          s[0] += a[k][j];
+          s[1] = fmaf(a[k][j], e.xh[j], s[1]);
+          s[2] += v[k][j];
+          s[3] = fmaf(v[k][j], e.xh[j], s[3]);
         }
       }
-#pragma unroll
-      for (int i = 0; i < K; ++i) s[i] += t[i];
     }
-    RowSums<256, K>::run(s, sm, turn);
+    RowSums<256, CURVED ? 2 : 4>::run(s, sm, turn);
+    if constexpr (!CURVED) {
+      const float count = (float)(p.cols - c0 < CHUNK ? p.cols - c0 : CHUNK), am = s[0] / count, vmean = s[2] / count;
+      float t[1] = {0.f};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int n = (int)(p.cols - c0) - (threadIdx.x + k * 256) * 8;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t[0] = fmaf(j < n ? v[k][j] - vmean : 0.f, a[k][j] - am, t[0]);
+      }
+      RowSums<256, 1>::run(t, sm2, turn2);
+      if (threadIdx.x == 0) p.chunk[item * K + 4] = t[0];
+    }
     if (threadIdx.x == 0)
 #pragma unroll
-      for (int i = 0; i < K; ++i) p.chunk[item * K + i] = s[i];
+      for (int i = 0; i < (CURVED ? 2 : 4); ++i) p.chunk[item * K + i] = s[i];
+  }
+}
+
+// 2 (ln_join for the sums of q gamma): sums of a row's chunks, joined by a wave; the last one = those around the chunks' means +
+// the means' own spread.
+__global__ __launch_bounds__(256) void ln_bwd2_join(LnArgs p, long chunks) {
+  const int lane = threadIdx.x & 63;
+  const float cols = (float)p.cols, last = (float)(p.cols - (chunks - 1) * CHUNK);
+  for (long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6); row < p.rows; row += (long)gridDim.x * 4) {
+    const float* part = p.chunk + row * chunks * 5;
+    float s[4] = {};
+    for (long i = lane; i < chunks; i += 64)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s[k] += part[i * 5 + k];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s[k] = lanes_sum<64>(s[k]);
+    const float am = s[0] / cols, vm = s[2] / cols;
+    float t = 0.f;
+    for (long i = lane; i < chunks; i += 64) {
+      const float n = i + 1 < chunks ? (float)CHUNK : last;
+      t += fmaf((part[i * 5 + 2] / n - vm) * n, part[i * 5] / n - am, part[i * 5 + 4]);
+    }
+    t = lanes_sum<64>(t);
+    if (lane == 0) {
+      float* out = p.row + row * ROW_SUMS;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) out[k] = s[k];
+      out[4] = t;
+    }
   }
 }
 
@@ -258,9 +307,9 @@ __global__ __launch_bounds__(256) void ln_bwd2_stream(LnArgs p) {
     const float mean = p.mean[row], rstd = p.rstd[row];
     const float* rs = p.row + row * ROW_SUMS;
     const float am = rs[0] * inv, ax = rs[1] * inv, vm = rs[2] * inv, vx = rs[3] * inv;
-    const float sv = rs[4] * inv - vm * am - vx * ax;
+    const float sv = rs[4] * inv - vx * ax;
     const float q0 = curved ? rs[5] * inv : 0.f, q1 = curved ? rs[6] * inv : 0.f;
-    const float c0 = rstd * (rstd * am * vx - q0), c1 = -rstd * ax, c2 = -rstd * rstd * vx;
+    const float c0 = -rstd * q0, c1 = -rstd * ax, c2 = -rstd * rstd * vx;
     const float c3 = -rstd * (q1 + rstd * (sv - vx * ax));
     e.make(p, row, c, mean, rstd, ga, be);
 #pragma unroll
@@ -268,7 +317,7 @@ __global__ __launch_bounds__(256) void ln_bwd2_stream(LnArgs p) {
       const float t = rstd * (v[j] - vm - e.xh[j] * vx);
       const float q = EPI == 2 ? e.g[j] * e.d2[j] * ga[j] * t : 0.f, g1 = EPI == 2 ? e.g[j] * e.d1[j] : e.g[j];
       gg[j] = (EPI == 2 ? e.d1[j] * ga[j] : ga[j]) * t;
-      gx[j] = fmaf(t, c1, fmaf(g1 * ga[j], c2, fmaf(e.xh[j], c3, c0)));
+      gx[j] = fmaf(t, c1, fmaf(fmaf(g1, ga[j], -am), c2, fmaf(e.xh[j], c3, c0)));
       dg[j] = fmaf(g1, t, dg[j]);
       if (EPI == 2) {
         gx[j] = fmaf(q * ga[j], rstd, gx[j]);
@@ -292,7 +341,7 @@ void launch_split(const LnArgs& a, hipStream_t st) {
   const long chunks = ln_chunks(a.cols);
   const unsigned items = ln_items(a.rows, a.cols);
   ln_bwd2_chunks<T, EPI, false><<<items, 256, 0, st>>>(a, chunks);
-  ln_join<5><<<ln_join_grid(a.rows), 256, 0, st>>>(a.chunk, a.rows, chunks, a.row, 0);
+  ln_bwd2_join<<<ln_join_grid(a.rows), 256, 0, st>>>(a, chunks);
   if (EPI == 2 && a.act > 1.f) {
     ln_bwd2_chunks<T, EPI, true><<<items, 256, 0, st>>>(a, chunks);
     ln_join<2><<<ln_join_grid(a.rows), 256, 0, st>>>(a.chunk, a.rows, chunks, a.row, 5);

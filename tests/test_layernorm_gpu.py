@@ -514,6 +514,41 @@ def test_split_rows(dev, rows, cols):
     run_all(dev, rows, cols, F16, 0.01, 0.4, seed=2)
 
 
+# ---- the second backward around its means -----------------------------------------------------------------------------------
+
+def offset_case(dev, rows, cols, dtype, offset, code, p, seed=0):
+    """First and second backward with gradients whose mean is ``offset`` times their spread, against bounds that grow with the
+    offset, not with its square."""
+    from fcd_amd import ops
+    t, _ = case(dev, rows, cols, dtype, seed=seed)
+    # (gamma's spread shrinks with the offset: that of gamma gy stays the noise's)
+    t["gamma"] = (1 + (t["gamma"].double() - 1) / offset).float()
+    t["gy"] = (t["gy"].double() + offset).to(dtype)
+    t["ggx"] = (t["ggx"].double() + offset).to(dtype)
+    d = {k: v.double() for k, v in t.items()}
+    m = mask_of(rows, cols, p)
+    m = None if m is None else m.to(dev)
+    kw = dict(act_slope=code, p=p, rng=(SEED, OFFSET) if p else None)
+    mean, rstd = ops.layernorm_fwd(t["x"], t["gamma"], t["beta"])[1:]
+    md, rd = mean.double()[:, None], rstd.double()[:, None]
+    got = ops.layernorm_bwd(t["gy"], t["x"], mean, rstd, t["gamma"], t["beta"], **kw)
+    for g, w, dt, name in zip(got, R.backward(d["x"], d["gy"], md, rd, d["gamma"], d["beta"], code, m), (dtype, F32, F32),
+                              ("dx", "dgamma", "dbeta")):
+        R.check(g, w, dt, name)
+    got = ops.layernorm_bwd2(t["ggx"], t["gy"], t["x"], mean, rstd, t["gamma"], t["beta"], **kw)
+    for g, w, dt, name in zip(got, R.second(d["ggx"], d["x"], d["gy"], md, rd, d["gamma"], d["beta"], code, m), (dtype, dtype, F32, F32),
+                              ("ggy", "gx", "dgamma of the second backward", "dbeta of the second backward")):
+        R.check(g, w, dt, name)
+
+
+@pytest.mark.parametrize("offset", [10.0, 100.0, 1000.0])
+@pytest.mark.parametrize("cols", [7, 24, 60, 100, 255, 500, 1001, 1537, 4096, 8192, 8195, 20000, 65541])
+def test_gradients_far_from_zero(dev, cols, offset):
+    for i, (code, p) in enumerate(((1.0, 0.0), (2.0, 0.0), (0.01, 0.3), (1.0, 0.3))):
+        offset_case(dev, 37 if cols < 9000 else 5, cols, F32, offset, code, p, seed=i)
+    offset_case(dev, 9, cols, BF16, offset, 1.0, 0.0)
+
+
 # ---- activations far out ----------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("code", [2.0, 3.0])
