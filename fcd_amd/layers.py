@@ -6,6 +6,8 @@ differentiating the parameters' gradients is refused.  Dropout masks are recompu
 reference counterpart: the reference's networks have neither.
 
 Capturing a backward pass into a HIP graph: let go of eager graphs over the same parameters first (as for any torch module).
+A forward pass that is run a second time (activation checkpointing) draws a new range of a module's generator, so its backward
+would belong to another mask: there call the functions, with an ``rng`` taken outside the part that is run again.
 """
 from __future__ import annotations
 
@@ -29,12 +31,25 @@ def _even(t: torch.Tensor) -> torch.Tensor:
         return t.contiguous()
 
 
+def _words(rng):
+    """(tensor, rest) of an ``rng``: its tensor is saved for the backward pass like an operand, so that autograd refuses one that
+    has changed by then."""
+    if isinstance(rng, torch.Tensor):
+        return rng, None
+    return tuple(rng) if rng is not None and isinstance(rng[0], torch.Tensor) else (None, rng)
+
+
+def _rng(words, rest):
+    return rest if words is None else words if rest is None else (words, rest)
+
+
 class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, eps, act, p, rng):
         y, mean, rstd = ops.layernorm_fwd(_even(x), weight, bias, eps, act, p, rng, None if residual is None else _even(residual))
-        ctx.save_for_backward(x, weight, bias, mean, rstd)      # (x itself, not a copy: the second backward leads to it)
-        ctx.cfg = act, p, rng
+        words, rest = _words(rng)
+        ctx.save_for_backward(x, weight, bias, mean, rstd, words)      # (x itself, not a copy: the second backward leads to it)
+        ctx.cfg = act, p, rest
         ctx.set_materialize_grads(False)
         return y
 
@@ -42,11 +57,12 @@ class _LayerNormFn(torch.autograd.Function):
     def backward(ctx, gy):
         if gy is None:
             return (None,) * 8
-        x, weight, bias, mean, rstd = ctx.saved_tensors
+        x, weight, bias, mean, rstd, words = ctx.saved_tensors
+        act, p, rest = ctx.cfg
         needs = ctx.needs_input_grad
         dx = dw = db = None
         if any(needs[:3]):
-            dx, dw, db = _LayerNormBwdFn.apply(gy, x, weight, bias, mean, rstd, ctx.cfg, bool(needs[1] or needs[2]))
+            dx, dw, db = _LayerNormBwdFn.apply(gy, x, weight, bias, mean, rstd, (act, p, _rng(words, rest)), bool(needs[1] or needs[2]))
         return (dx if needs[0] else None, dw if needs[1] else None, db if needs[2] else None, gy if needs[3] else None,
                 None, None, None, None)
 
@@ -58,8 +74,9 @@ class _LayerNormBwdFn(torch.autograd.Function):
     def forward(ctx, gy, x, weight, bias, mean, rstd, cfg, want_affine):
         gy, x = _even(gy), _even(x)
         act, p, rng = cfg
-        ctx.save_for_backward(gy, x, weight, bias, mean, rstd)
-        ctx.cfg = cfg
+        words, rest = _words(rng)
+        ctx.save_for_backward(gy, x, weight, bias, mean, rstd, words)
+        ctx.cfg = act, p, rest
         ctx.set_materialize_grads(False)
         return ops.layernorm_bwd(gy, x, mean, rstd, weight, bias, act, p, rng, want_affine=want_affine)
 
@@ -70,10 +87,10 @@ class _LayerNormBwdFn(torch.autograd.Function):
             raise NotImplementedError("differentiating through a layer norm's parameter gradients is not supported")
         if ggx is None:
             return (None,) * 8
-        gy, x, weight, bias, mean, rstd = ctx.saved_tensors
-        act, p, rng = ctx.cfg
+        gy, x, weight, bias, mean, rstd, words = ctx.saved_tensors
+        act, p, rest = ctx.cfg
         needs = ctx.needs_input_grad
-        ggy, gx, dw, db = ops.layernorm_bwd2(_even(ggx), gy, x, mean, rstd, weight, bias, act, p, rng,
+        ggy, gx, dw, db = ops.layernorm_bwd2(_even(ggx), gy, x, mean, rstd, weight, bias, act, p, _rng(words, rest),
                                              want_affine=bool(needs[2] or needs[3]))
         return ggy, gx, dw if needs[2] else None, db if needs[3] else None, None, None, None, None
 
@@ -81,13 +98,16 @@ class _LayerNormBwdFn(torch.autograd.Function):
 class _DropoutFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, p, rng, residual):
-        ctx.cfg = p, rng
+        words, rest = _words(rng)
+        ctx.save_for_backward(words)
+        ctx.cfg = p, rest
         return ops.dropout(_even(x), p, rng, None if residual is None else _even(residual))
 
     @staticmethod
     def backward(ctx, gy):
-        p, rng = ctx.cfg
+        p, rest = ctx.cfg
         needs = ctx.needs_input_grad
+        rng = _rng(ctx.saved_tensors[0], rest)
         return _DropoutFn.apply(gy, p, rng, None) if needs[0] else None, None, None, gy if needs[3] else None
 
 

@@ -833,6 +833,8 @@ def dropout_take(state: torch.Tensor, numel: int) -> torch.Tensor:
         raise RuntimeError("fcd_amd: dropout_take of a negative number of elements")
     taken = torch.empty_like(state)
     check(L.load().fcd_dropout_take(state.data_ptr(), taken.data_ptr(), (int(numel) + 7) // 8, stream()), "dropout_take")
+    if not state.is_inference():
+        torch.autograd.graph.increment_version(state)      # written by a raw kernel: a graph that saved it finds out
     return taken
 
 

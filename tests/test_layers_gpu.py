@@ -329,3 +329,27 @@ def test_modules_without_a_seed_drop_other_elements(dev):
         for i in range(3):
             for k in range(i):
                 assert abs(float((kept[i] == kept[k]).double().mean()) - 0.5) <= 6 * (0.25 / x.numel()) ** 0.5
+
+
+def test_rng_that_changed_since_the_forward_pass(dev):
+    """The backward passes draw the forward's mask again: an rng tensor that moved on meanwhile (a generator's own state, or words
+    written over) is refused as any saved tensor is, not used for another mask."""
+    from fcd_amd import layers, ops
+    x = torch.randn(16, 64, device=dev, requires_grad=True)
+    moves = {"state": lambda t: ops.dropout_take(t, x.numel()), "words": lambda t: t.add_(1)}
+    for move in moves.values():
+        for wrap in (lambda t: t, lambda t: (t, 5)):
+            for run in (lambda rng: layers.dropout(x, 0.5, rng), lambda rng: layers.layer_norm(x, activation="silu", p=0.5, rng=rng)):
+                rng = ops.dropout_state(3, dev)
+                y = run(wrap(rng))
+                want, = torch.autograd.grad(y, x, torch.ones_like(y), retain_graph=True)       # (unchanged: taken)
+                assert torch.equal(want, torch.autograd.grad(y, x, torch.ones_like(y), retain_graph=True)[0])
+                move(rng)
+                with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                    torch.autograd.grad(y, x, torch.ones_like(y))
+                gy = torch.ones_like(y).requires_grad_(True)
+                rng = ops.dropout_state(3, dev)
+                dx, = torch.autograd.grad(run(wrap(rng)), x, gy, create_graph=True)
+                move(rng)
+                with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                    torch.autograd.grad(dx, gy, torch.ones_like(dx))
