@@ -7,13 +7,13 @@ import numpy as np
 import torch
 
 U = 2.0 ** -24            # half a step of fp32, relative
-# Additions on the longest path of one row sum: 8 elements of a lane, at most 64 lane steps of the tested lengths, 6 stages
-# in the wave, up to 16 waves one after another, and the division by the length.
+# Additions on the longest path of one row sum: 8 elements of a lane's unit, up to 64 units or chunks one after another at the
+# tested lengths, 6 stages in the wave, up to 16 waves, and the division by the length.
 CHAIN = 8 + 64 + 6 + 16 + 1
-# ... of a column sum: at most 16 rows kept by a thread of the tested sizes' workgroups times up to 64 threads of one
-# column, then up to 256 workgroups in four strands of 64 and a join.
+# ... of a column sum: up to 80 rows kept by a thread and the wave's threads of that column, up to 16 wave sums one after another,
+# then up to 512 workgroups' sums in at most 32 strands of 16, joined in order (48).
 COLUMN = 80 + 64 + 64 + 4
-FUNC = 16                 # an activation or its derivatives: a few roundings around expf / log1pf / tanhf of 1-2 steps each
+FUNC = 16                 # an activation or its derivatives: a few roundings around an exp2 and reciprocals of a step each
 
 
 class V:
