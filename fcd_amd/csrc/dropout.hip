@@ -8,9 +8,10 @@ namespace {
 // generator's blocks, not at the row's first element (memory takes any alignment; half a block would cost a whole one), so
 // that a row's first unit may begin late and its last end early.  256 threads a row (WIDE), or 2^lt of them and several rows
 // a workgroup; a tensor without gaps is one long row.
-// Bound by memory, 16384 x 8192 bf16 95 us (5.7 TB/s; a large copy runs at 5.1), with a residual 137 (5.9), at 17 vector
-// instructions an element.  Rows that start anywhere in a block, 16384 x 8191 in rows of 8192: 133 (150 with units that start
-// at the row and draw two blocks each).  65536 x 64 fp32 in rows of 68: 8 (35 with a workgroup per row).
+// Bound by memory, 16384 x 8192 bf16 95 us (5.7 TB/s), with a residual 134 (6.0, as without dropout: the best that a stream
+// reads and writes here), at 17 vector instructions an element.  Rows that start anywhere in a block, 16384 x 8191 in rows of
+// 8192: 132, of which 125 without dropout, for unaligned units and rows' ends (150 with units that start at the row and draw two
+// blocks each).  65536 x 64 fp32 in rows of 68: 8 (35 with a workgroup per row).
 template <typename T, bool WIDE>
 __global__ __launch_bounds__(256) void dropout_kernel(const T* x, const T* res, T* y, long rows, long cols, long ld_x,
                                                       long ld_res, long ld_y, int lt, Drop d) {

@@ -5,10 +5,10 @@ namespace {
 
 // A row's x and gy in registers, one exchange for both of its sums, dx out; a thread meets the same columns in every row, so
 // the affine sums stay in its registers until the last row.  The next row's loads are in flight meanwhile.  One unit of 8
-// columns a thread leaves four waves a SIMD and the registers for it; two units, two waves and no prefetch took 244 us for
-// 16384 x 8192 bf16 dropout where one took 174 (143 to 146 now).
-// Bound by memory, 16384 x 8192 bf16 144 us (5.6 TB/s), 4096 x 4096 19.5, 65536 x 64 fp32 10.2 (with dropout the
-// vector ALU is 64 % active at 16384 x 8192).  The affine join behind it: 4 to 7 us.
+// columns a thread leaves the registers for it (1024 threads are four waves a SIMD, shorter rows get two: ln_groups); two units,
+// two waves and no prefetch took 244 us for 16384 x 8192 bf16 dropout where one took 174 (141 to 188 now, by the process).
+// Bound by memory, 16384 x 8192 bf16 146 us (5.5 TB/s), 4096 x 4096 19.3, 65536 x 64 fp32 10.2 (with dropout the
+// vector ALU is 67 % active at 16384 x 8192).  The affine join behind it: 4 to 7 us.
 // EPI 0: plain; 1: dropout; 2: activation, and dropout if there is any.
 // (`blocks` workgroups from the first on; AFFINE: the affine sums are kept.)
 template <typename T, int G, int NV, int EPI, bool AFFINE>

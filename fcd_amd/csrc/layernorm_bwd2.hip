@@ -9,8 +9,8 @@ namespace {
 // 44 us, 2048 x 8192 behind a leaky slope 37.7 -> 39.7.  Waves that centre on their own means and join them in the first one:
 // equal or slower, and spilt.)
 // With the row's sums in hand gx is a combination of four things: c0 + c1 t + c2 a + c3 xhat (+ rstd q gamma).
-// Bound by memory without an activation, 16384 x 8192 bf16 245 us (5.5 TB/s), 4096 x 4096 29, 65536 x 64 fp32 15.6; with SiLU and
-// dropout by the vector ALU (81 % active at 4096 x 4096 bf16, 40 us).  Four waves a SIMD by force spill: 65536 x 64 fp32 SiLU
+// Bound by memory without an activation, 16384 x 8192 bf16 245 us (5.5 TB/s), 4096 x 4096 29, 65536 x 64 fp32 16; with SiLU and
+// dropout by the vector ALU (79 % active at 4096 x 4096 bf16, 39 to 41 us).  Four waves a SIMD by force spill: 65536 x 64 fp32 SiLU
 // 17.6 -> 34.6 us.
 // EPI 0: plain; 1: dropout; 2: activation, and dropout if there is any.
 template <typename T, int G, int NV, int EPI>
@@ -197,7 +197,7 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void ln_bwd2_rows(LnArgs p) {
 
 // Split rows, 1: a chunk's sums of a, a xhat, v and v xhat, and that of (v - its mean) (a - its mean) around the chunk's own
 // means; with the joined ones known and a curved activation (CURVED) the two sums of q gamma.
-// All kernels of a call: 4096 x 12288 bf16 210 us (one workgroup per row that read it again: 489), 8 x 262144 fp32 32.
+// All kernels of a call: 4096 x 12288 bf16 214 us (one workgroup per row that read it again: 489), 8 x 262144 fp32 32.
 template <typename T, int EPI, bool CURVED>
 __global__ __launch_bounds__(256) void ln_bwd2_chunks(LnArgs p, long chunks) {
   constexpr int K = CURVED ? 2 : 5;

@@ -7,9 +7,9 @@ namespace {
 // rows far from zero), then the result.  A workgroup walks over rows with its columns' parameters in registers (fp32 gamma and
 // beta are four times a bf16 row) and the next row's loads in flight; the grid is eight waves a SIMD (half of it: 65536 x 1024
 // bf16 42.8 -> 44.7 us), or one workgroup of 1024, of which no second one fits (2048 x 12288 bf16 dropout with two 28.6, 26.4).
-// Bound by memory: 16384 x 8192 bf16 95 us (5.6 TB/s; a large copy runs at 5.1), with dropout 97 to 116 from
-// process to process; 4096 x 4096 13.3, with SiLU and dropout 19.6; 8192 x 2048 with dropout 16.8; 65536 x 64 fp32 7.9, with
-// leaky ReLU and dropout 8.5.  16384 x 8192 with dropout and a residual takes 23
+// Bound by memory: 16384 x 8192 bf16 95 us (5.6 TB/s; the best stream that reads and writes runs at 6.0), with dropout 97 to 116
+// from process to process; 4096 x 4096 14, with SiLU and dropout 19.6; 8192 x 2048 with dropout 16.6; 65536 x 64 fp32 6.9, with
+// leaky ReLU and dropout 7.8.  16384 x 8192 with dropout and a residual takes 23
 // vector instructions an element, most of them the generator's.
 template <typename T, int G, int NV, bool EPI>
 __global__ __launch_bounds__(G > 64 ? G : 256) void ln_fwd_rows(LnArgs p) {

@@ -235,8 +235,8 @@ class FCDSolver(nn.Module):
                  "fp32x2": (L.PREC_F16X2, None), "fp16": (L.PREC_F16, None)}[precision]
         for net in (self.G, self.D):
             if net is self.D and p in L.F16_FAMILY and (self.D.smooth or not self.d_scaled_fp16):
-                # SiLU / Mish discriminators keep their un-fused activation launches and no maxima bookkeeping: split bf16
-                # pieces under fp32x2, plain bf16 operands under the reduced-precision variant
+                # discriminators with SiLU / Mish, a norm or dropout keep their un-fused launches and no maxima bookkeeping:
+                # split bf16 pieces under fp32x2, plain bf16 operands under the reduced-precision variant
                 net.precision = L.PREC_BF16X3 if p == L.PREC_F16X2 else L.PREC_BF16
             else:
                 net.precision = p
@@ -380,8 +380,9 @@ class FCDSolver(nn.Module):
 
                 if self.use_feats or not self._in_train_step or not self.skip_unused_d_forward:
                     _, _, x_reconst_id_feats = self.D(x_reconst_id)    # reference :358
-                # (else: the reference computes this forward and drops its outputs -- only use_feats reads them, D has
-                #  no buffers, nothing requires its graph: a dead call, left out by train_step)
+                # (else: the reference computes this forward and drops its outputs -- only use_feats reads them, nothing
+                #  requires its graph, and D's only buffer is the state of its dropout, which the reference has not: a dead
+                #  call, left out by train_step)
                 g_loss_rec_id = losses.l1_mean(x_real, x_reconst_id)
 
                 if self.use_feats:
