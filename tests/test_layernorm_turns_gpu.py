@@ -143,3 +143,34 @@ def test_dropout_in_place_with_rows_inside_a_block(dev, rows, cols, dtype):
     got = ops.dropout(wide[:, :cols], 0.3, (SEED, OFFSET), out=wide[:, :cols])
     R.check(got, R.V(want, 2 * R.U * want.abs()), dtype)
     assert torch.equal(got == 0, want == 0) and torch.equal(wide[:, cols:], tail)
+
+
+@pytest.mark.parametrize("rows,cols", [(525000, 8192), (67200000, 64), (140000, 32768)])
+def test_more_than_4_billion_elements(dev, rows, cols):
+    """Register-resident and split rows beyond 2^32 elements: the first, a middle and the last rows have the bits that the same rows
+    have by themselves, in all three directions and in dropout, written over their inputs to keep the memory small."""
+    from fcd_amd import ops
+    g = torch.Generator(device=dev).manual_seed(1)
+    few = 24
+    at = [0, rows // 2 // 8 * 8, rows - few]
+    tile = [torch.randn(few, cols, generator=g, device=dev).to(BF16) for _ in range(3)]
+    x, gy, v = (t.repeat((rows + few - 1) // few, 1)[:rows] for t in tile)
+    samples = [[t[i:i + few].clone() for i in at] for t in (x, gy, v)]
+    kw = dict(act_slope=2.0, p=0.25)
+    y = torch.empty_like(x)
+    _, mean, rstd = ops.layernorm_fwd(x, out=y, rng=(3, 4), **kw)
+    want = [ops.layernorm_fwd(s, rng=(3, 4 + i * cols // 8), **kw) for s, i in zip(samples[0], at)]
+    for i, w in zip(at, want):
+        assert torch.equal(y[i:i + few], w[0]) and torch.equal(mean[i:i + few], w[1]) and torch.equal(rstd[i:i + few], w[2])
+    ops.layernorm_bwd(gy, x, mean, rstd, out=y, rng=(3, 4), **kw)
+    for k, i in enumerate(at):
+        w = ops.layernorm_bwd(samples[1][k], samples[0][k], *want[k][1:], rng=(3, 4 + i * cols // 8), **kw)[0]
+        assert torch.equal(y[i:i + few], w)
+    del y
+    ops.layernorm_bwd2(v, gy, x, mean, rstd, outs=(gy, v), rng=(3, 4), **kw)
+    for k, i in enumerate(at):
+        w = ops.layernorm_bwd2(samples[2][k], samples[1][k], samples[0][k], *want[k][1:], rng=(3, 4 + i * cols // 8), **kw)
+        assert torch.equal(gy[i:i + few], w[0]) and torch.equal(v[i:i + few], w[1])
+    ops.dropout(x, 0.25, (3, 4), out=x)
+    for k, i in enumerate(at):
+        assert torch.equal(x[i:i + few], ops.dropout(samples[0][k], 0.25, (3, 4 + i * cols // 8)))
